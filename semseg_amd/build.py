@@ -8,7 +8,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OBJ = os.path.join(HERE, 'csrc', 'build')
 LIB = os.path.join(HERE, 'libsemseg_hip.so')
-FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=fast', '-Wno-unused-result']
+# fast-honor-pragmas: contraction everywhere but where a kernel says `#pragma clang fp contract(off)` (plain `fast` ignores it);
+# no packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on gfx950
+FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=fast-honor-pragmas', '-Wno-unused-result',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def _newer(src, dst, deps):
