@@ -381,6 +381,10 @@ __global__ __launch_bounds__(256) void lawin_attn_bwd_kernel(const T* __restrict
         store_d<T, D, VEC>(dtheta + row * lddt + hd * D, acc);
     }
     T* drow = dpg + (wi * 64 + lane) * (2 * (int64_t)inter) + hd * D;
+    // pass B reads this lane's phi and g rows again from LDS: held in registers across pass A they take the D = 64 kernel past 512 (spills)
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int d = 0; d < D; ++d) { pk[d] = ph[lane * D + d]; gk[d] = gg[lane * D + d]; }
     {   // pass B, lane = key: dg_k = sum_q p dY_q ; dphi_k = scale * sum_q p (dp - delta_q) theta_q   (ts holds theta*c2: undone at the end)
         float ag[D], ap[D];
 #pragma unroll
