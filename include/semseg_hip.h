@@ -561,6 +561,59 @@ int ss_image_affine(int out_dtype, const float* in, int64_t ldi, const float* M,
 int ss_adabound_step(float* p, const float* g, float* m, float* v, int64_t n, double beta1, double beta2, float eps,
                      float step_size, float lower, float upper, float weight_decay, float grad_scale, hipStream_t stream);
 
+/* ---- the residual update between two blocks with a norm on either side of it (LayerScale / gated / sandwich-norm residual blocks; the
+ * reference has the plain form x + drop_path(gamma * f(norm(x))), modules/convnext.py:38-51, modules/segformer.py:94-98):
+ *   n = post(b);  h = alpha x + keep[s] scale[c] act(gate) n;  y = pre(h)        rows r of sample s = r / rows_per_sample, C <= 4096 channels
+ * post, pre: 0 none, 1 LayerNorm (weight, bias may be NULL), 2 RMSNorm (weight); gate_mode: 0 none, 1 one row of C per sample, 2 one per row;
+ * act: 0 identity, 1 sigmoid.  x and h have x_dtype, b, gate and y b_dtype: f32 / f32, bf16 / bf16 or f32 / bf16.  x, b, gate (and the
+ * backward's dh, dy, h) have unit inner stride and their own row stride, aligned to the element only; h, y, dx, db, dgate are dense.  y is
+ * computed from h as stored.  scale, keep, the weights and the vectors' gradients are float.  stats [rows][4] (optional in the forward): mean
+ * and 1 / deviation of b and of h.  Any width of rows, none of them aligned, is taken.  h may not overlap an input. */
+int ss_resnorm_fwd(int x_dtype, int b_dtype, const void* x, int64_t ldx, const void* b, int64_t ldb, const void* gate, int64_t ldg, int gate_mode,
+                   int act, const float* scale, const float* keep, float alpha, int post, const float* post_w, const float* post_b, int pre,
+                   const float* pre_w, const float* pre_b, double eps, void* h, void* y, float* stats, int64_t rows, int64_t rows_per_sample,
+                   int C, hipStream_t stream);
+int64_t ss_resnorm_bwd_workspace(int64_t rows, int64_t rows_per_sample, int C, int post, int pre, int gate_mode, int has_scale);
+/* dh and dy: gradients of h and of y, either may be NULL (h is read only with dy).  dgate as the gate.  dvec: float, one row of C per existing
+ * vector, in this order: pre weight, pre bias (LayerNorm), post weight, post bias (LayerNorm), scale.  Sums run in a fixed order. */
+int ss_resnorm_bwd(int x_dtype, int b_dtype, const void* dh, int64_t lddh, const void* dy, int64_t lddy, const void* h, int64_t ldh,
+                   const void* b, int64_t ldb, const void* gate, int64_t ldg, int gate_mode, int act, const float* scale, const float* keep,
+                   float alpha, int post, const float* post_w, const float* post_b, int pre, const float* pre_w, const float* stats, void* dx,
+                   void* db, void* dgate, float* dvec, int64_t rows, int64_t rows_per_sample, int C, float* workspace, int64_t ws_bytes,
+                   hipStream_t stream);
+
+/* ---- AdamW (Loshchilov & Hutter 2019) over many tensors in one launch, with the global gradient norm and clipping; moments in 32 bits or
+ * in 8.  The reference trains with AdaBound only (train.py:53-58); this is the optimizer that the published recipes of its encoders use.
+ *   g' = coef g;  m = b1 m + (1-b1) g';  v = b2 v + (1-b2) g'^2;  p = (1 - lr wd) p - lr / (1-b1^t) m / (sqrt(v) / sqrt(1-b2^t) + eps)
+ *   coef = grad_scale min(1, max_norm / (norm + 1e-6)),  norm = grad_scale |all gradients| (squares summed in double)
+ * Tensors are given as HOST arrays of device addresses (params, grads; contiguous, aligned to their element) and a PLAN in device memory
+ * that holds no address: one record of four 64-bit words per chunk of a tensor,
+ *   { first element in the tensor;  elements | first run << 32;  tensor | group << 32;  0 },
+ * chunks in tensor order, each of at most 2^20 elements, a multiple of 256 but for a tensor's last; first_chunk[count + 1] (HOST) says
+ * where each tensor's records begin.  A NULL gradient leaves its tensor and moments as they are.  A RUN is 256 elements of one tensor (its last may be shorter); the state holds whole runs:
+ *   bits 32: m and v are float[runs * 256];  bits 8: m is int8 codes c (sign(c) c^2 q), v is uint8 codes c (c^4 q), both [runs * 256],
+ *   and m_scale / v_scale are the q, float[runs].  Codes are drawn between the two neighbours so that their mean is the moment (hash of
+ *   seed, t, run, element); a positive second moment never takes code 0; moments below 1e-28 are held as zero; a NaN or infinite moment
+ *   makes its run NaN.  The parameter is updated from the moments before they are rounded.
+ * lr and weight_decay are HOST arrays of `groups` <= 64 doubles.  `dyn` (device, ss_adamw_dyn_workspace() bytes), when given, holds what
+ * ss_adamw_prepare left there and stands in for grad_scale, t, lr, weight_decay and seed. */
+int ss_multi_sqnorm(int dtype, int count, const void* const* grads, const int64_t* first_chunk, const void* plan, double* partial /* [chunks] */,
+                    hipStream_t stream);
+int64_t ss_adamw_dyn_workspace(void);
+/* One workgroup: norm from the partial sums (may be none), clipping coefficient, bias corrections and learning rates into `dyn`.  t_dev, when
+ * given, is the step count on the device: it is advanced by one and used instead of t (a captured graph counts its replays so); lr_dev, when
+ * given, is double[groups] on the device and read instead of lr.  max_norm <= 0: no clipping.  skip_nonfinite: with a norm that is infinite or
+ * NaN the step count stays and ss_adamw_step changes nothing. */
+int ss_adamw_prepare(const double* partial, int64_t chunks, double max_norm, double grad_scale, double beta1, double beta2, int64_t t,
+                     int64_t* t_dev, int groups, const double* lr, const double* weight_decay, const double* lr_dev, int64_t seed,
+                     int skip_nonfinite, float* norm, void* dyn, hipStream_t stream);
+int ss_adamw_step(int p_dtype, int g_dtype, int bits, int count, void* const* params, const void* const* grads, const int64_t* first_chunk,
+                  const void* plan, void* m, void* v, float* m_scale, float* v_scale, double beta1, double beta2, double eps, double grad_scale,
+                  int64_t t, int groups, const double* lr, const double* weight_decay, int64_t seed, const void* dyn, hipStream_t stream);
+/* the moments that the 8-bit codes of `runs` runs stand for, as floats */
+int ss_adamw8_values(const void* m, const void* v, const float* m_scale, const float* v_scale, float* m_out, float* v_out, int64_t runs,
+                     hipStream_t stream);
+
 /* ---- gradient delivery: dst[i][0..numel[i]) += src[i] for `count` fp32 tensors in one launch per 40 tensors.  Source i is
  * numel[i] / cols[i] rows of cols[i] contiguous floats, src_ld[i] apart (cols[i] == numel[i]: contiguous); dst[i] is contiguous.
  * src, src_ld, cols, dst and numel are HOST arrays.  Replaces autograd's per-parameter AccumulateGrad adds (what DDP's reducer

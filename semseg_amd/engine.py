@@ -10,8 +10,11 @@ in the reference, laid out for one process per MI355X:
   post-accumulate-grad hooks the moment its last gradient has been produced, on a side stream, so the exchange of bucket
   k overlaps the backward kernels of bucket k+1; ``wait()`` joins them before the optimizer.  SUM is used and the 1/world
   mean is folded into the optimizer kernel's ``grad_scale``;
-* ``AdaBound``  is one HIP launch over the flat buffers (``ss_adabound_step``).
+* ``AdaBound``  is one HIP launch over the flat buffers (``ss_adabound_step``);
+* ``AdamW``  is the optimizer of the encoders' published recipes (``ss_adamw_step``): flat buffers or a list of tensors, moments in 32 or 8
+  bits, gradient clipping by the global norm inside the step.
 """
+import ctypes
 import math
 import torch
 import torch.distributed as dist
@@ -299,6 +302,208 @@ class AdaBound:
         if len(steps) > 1:
             raise ValueError(f'AdaBound.load_state_dict: parameters at different steps {sorted(steps)}; one flat step count is kept')
         self.t = steps.pop() if steps else 0
+
+
+class AdamW:
+    """AdamW (Loshchilov & Hutter 2019; torch.optim.AdamW's arithmetic) over many tensors in one launch, with clipping by the global gradient
+    norm inside the step and the moments in 32 or in 8 bits.
+
+    ``params``: ``FlatParams`` (one address for the whole model), or an iterable of float32 / bfloat16 parameters of one type on one device
+    whose ``.grad`` (any of the two types, one for all) is read at each step; a parameter without a gradient keeps its value and moments.
+    ``per_param``: callable, parameter -> dict with ``weight_decay`` and / or ``lr_scale`` of its own (norms and biases without decay,
+    layer-wise rates), at most 64 different ones.  ``max_grad_norm``: gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)), norm over
+    all of them after ``grad_scale``; ``step()`` then returns the norm (a device scalar, nothing waits for it).  ``state_bits=8``: a moment
+    is an 8-bit code with one scale per 256 elements, stored by a draw between two neighbours that depends on (seed, step, element)
+    only: 16 instead of 28 bytes per parameter and step.  ``skip_nonfinite``: a step whose gradient norm is infinite or NaN changes nothing
+    and is not counted.  ``capturable``: ``step()`` may be captured into a graph; the step count lives on the device, the learning rate
+    is read from there too (``push_lr()`` after moving ``lr`` between replays; betas and decay are captured as they are).  After replays call
+    ``weightprep.bump()``: the parameters were written behind torch's back.
+
+    ``lr`` and ``betas`` are plain attributes a scheduler may move (``OneCycleLR``)."""
+
+    MAX_GROUPS = 64
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=None, state_bits=32, seed=0, per_param=None,
+                 skip_nonfinite=False, capturable=False):
+        self.flat = params if isinstance(params, FlatParams) else None
+        self.params = list(self.flat.params if self.flat is not None else params)
+        if not self.params:
+            raise ValueError('AdamW: no parameters')
+        p0 = self.params[0]
+        self.device, self.dtype = p0.device, p0.dtype
+        for p in self.params:
+            if p.dtype != self.dtype or p.device != self.device or p.dtype not in (torch.float32, torch.bfloat16) or not p.is_contiguous():
+                raise ValueError('AdamW: parameters must be contiguous, of one type (float32 or bfloat16) and on one device')
+        if len({id(p) for p in self.params}) != len(self.params):
+            raise ValueError('AdamW: a parameter appears twice')
+        if state_bits not in (8, 32):
+            raise ValueError(f'AdamW: state_bits must be 8 or 32, got {state_bits}')
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0) or lr < 0.0 or eps < 0.0 or weight_decay < 0.0:
+            raise ValueError('AdamW: betas must lie in [0, 1), lr, eps and weight_decay must not be negative')
+        if max_grad_norm is not None and not max_grad_norm > 0.0:
+            raise ValueError('AdamW: max_grad_norm must be positive, or None')
+        self.lr, self.betas, self.eps, self.wd = lr, tuple(betas), eps, weight_decay
+        self.max_grad_norm, self.state_bits, self.seed = max_grad_norm, state_bits, int(seed) & 0xFFFFFFFF
+        self.skip_nonfinite, self.capturable = bool(skip_nonfinite), bool(capturable)
+        self.groups, of = [], []                               # (lr_scale, weight_decay) pairs; None: follow the optimizer's
+        for p in self.params:
+            own = per_param(p) if per_param is not None else {}
+            if set(own) - {'lr_scale', 'weight_decay'}:
+                raise ValueError(f'AdamW: per_param knows lr_scale and weight_decay, got {sorted(own)}')
+            key = (float(own.get('lr_scale', 1.0)), own.get('weight_decay'))
+            if key not in self.groups:
+                self.groups.append(key)
+            of.append(self.groups.index(key))
+        if len(self.groups) > self.MAX_GROUPS:
+            raise ValueError(f'AdamW: {len(self.groups)} different per-parameter settings, at most {self.MAX_GROUPS}')
+        self.group_of, self.numels = of, [p.numel() for p in self.params]
+        self.plan = ops.TensorPlan(self.numels, self.device, of, self.flat.offsets if self.flat is not None else None)
+        n, runs = self.plan.runs * ops.ADAMW_RUN, self.plan.runs
+        m_type, v_type = (torch.float32, torch.float32) if state_bits == 32 else (torch.int8, torch.uint8)
+        self.exp_avg = torch.zeros(n, dtype=m_type, device=self.device)
+        self.exp_avg_sq = torch.zeros(n, dtype=v_type, device=self.device)
+        self.exp_avg_scale = torch.zeros(runs, device=self.device) if state_bits == 8 else None
+        self.exp_avg_sq_scale = torch.zeros(runs, device=self.device) if state_bits == 8 else None
+        on_device = self.capturable or self.skip_nonfinite
+        self._t = 0
+        self._t_dev = torch.zeros(1, dtype=torch.int64, device=self.device) if on_device else None
+        self._lr_dev = torch.zeros(len(self.groups), dtype=torch.float64, device=self.device) if self.capturable else None
+        if self.capturable:
+            self.push_lr()
+
+    @property
+    def t(self):
+        """Steps taken (waits for the device where the count lives there)."""
+        return self._t if self._t_dev is None else int(self._t_dev.item())
+
+    @t.setter
+    def t(self, value):
+        self._t = int(value)
+        if self._t_dev is not None:
+            self._t_dev.fill_(self._t)
+
+    def _rates(self):
+        return [self.lr * s for s, _ in self.groups]
+
+    def push_lr(self):
+        """Copies ``lr`` to the device, where captured steps read it."""
+        if self._lr_dev is None:
+            raise RuntimeError('AdamW.push_lr: only with capturable=True')
+        self._lr_dev.copy_(torch.tensor(self._rates(), dtype=torch.float64))
+
+    def _addresses(self):
+        """-> gradient type, HOST arrays of the parameters' and gradients' addresses"""
+        if self.flat is not None:
+            f = self.flat
+            return torch.float32, self.plan.pointers(f.data.data_ptr()), self.plan.pointers(f.grad.data_ptr())
+        gt, pa, ga = None, [], []
+        for p, n in zip(self.params, self.numels):
+            g = p.grad
+            if p.dtype != self.dtype or p.device != self.device or p.numel() != n or not p.is_contiguous():
+                raise RuntimeError('AdamW: a parameter changed its type, device, size or layout')
+            pa.append(p.data_ptr())
+            if g is None:
+                ga.append(None)
+                continue
+            if gt is None:
+                gt = g.dtype
+            if g.dtype != gt or gt not in (torch.float32, torch.bfloat16) or g.device != self.device or g.numel() != n or not g.is_contiguous():
+                raise RuntimeError('AdamW: gradients must be contiguous, of one type (float32 or bfloat16) and on the parameters\' device')
+            ga.append(g.data_ptr())
+        return gt or torch.float32, self.plan.pointers(*pa), self.plan.pointers(*ga)
+
+    def step(self, grad_scale=1.0):
+        if self.device.type != 'cuda':
+            raise RuntimeError('semseg_amd.AdamW: parameters must live on a HIP device (no CPU fallback)')
+        gt, pa, ga = self._addresses()
+        plan, lb, norm, dyn = self.plan, lib(), None, None
+        k = len(self.groups)
+        lr = (ctypes.c_double * k)(*self._rates())
+        wd = (ctypes.c_double * k)(*[self.wd if w is None else w for _, w in self.groups])
+        b1, b2 = self.betas
+        with torch.cuda.device(self.device):
+            stream = torch.cuda.current_stream().cuda_stream
+            measured = self.max_grad_norm is not None or self.skip_nonfinite
+            if self._t_dev is None:
+                self._t += 1
+            if measured or self._t_dev is not None:
+                partial = torch.empty(plan.chunks if measured else 0, dtype=torch.float64, device=self.device)
+                dyn = torch.empty(lb.ss_adamw_dyn_workspace(), dtype=torch.uint8, device=self.device)
+                if measured:
+                    norm = torch.empty((), dtype=torch.float32, device=self.device)
+                    check(lb.ss_multi_sqnorm(ops._DT[gt], plan.count, ga, plan.first_chunk, plan.table.data_ptr(), partial.data_ptr(), stream))
+                check(lb.ss_adamw_prepare(partial.data_ptr(), partial.numel(), self.max_grad_norm or 0.0, grad_scale, b1, b2, self._t,
+                                          ops._p(self._t_dev), k, lr, wd, ops._p(self._lr_dev), self.seed, int(self.skip_nonfinite), ops._p(norm),
+                                          dyn.data_ptr(), stream))
+            check(lb.ss_adamw_step(ops._DT[self.dtype], ops._DT[gt], self.state_bits, plan.count, pa, ga, plan.first_chunk, plan.table.data_ptr(),
+                                   self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), ops._p(self.exp_avg_scale), ops._p(self.exp_avg_sq_scale), b1, b2,
+                                   self.eps, grad_scale, self._t, k, lr, wd, self.seed, ops._p(dyn), stream))
+        weightprep.bump()                                      # the kernel wrote the parameters through a raw pointer
+        return norm
+
+    def state_values(self):
+        """-> both moments as float32, in the state's layout (whole runs of 256 per parameter)"""
+        if self.state_bits == 32:
+            return self.exp_avg, self.exp_avg_sq
+        with torch.cuda.device(self.device):
+            m = torch.empty(self.exp_avg.numel(), device=self.device)
+            v = torch.empty(self.exp_avg.numel(), device=self.device)
+            check(lib().ss_adamw8_values(self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), self.exp_avg_scale.data_ptr(), self.exp_avg_sq_scale.data_ptr(),
+                                         m.data_ptr(), v.data_ptr(), self.plan.runs, torch.cuda.current_stream().cuda_stream))
+        return m, v
+
+    # ---- checkpointing in torch.optim's layout, parameters in registration order (FlatParams keeps them reversed); with 8-bit moments the
+    # codes and, per parameter, the scales of its runs
+    def _slots(self):
+        n = len(self.params)
+        for j, p in enumerate(self.params):
+            yield (n - 1 - j if self.flat is not None else j), j, p, self.plan.first_run[j], -(-self.numels[j] // ops.ADAMW_RUN)
+
+    def state_dict(self):
+        state, t = {}, self.t
+        for idx, _, p, run, runs in self._slots():
+            o, n = run * ops.ADAMW_RUN, p.numel()
+            state[idx] = {'step': t, 'exp_avg': self.exp_avg[o:o + n].view(p.shape).clone(), 'exp_avg_sq': self.exp_avg_sq[o:o + n].view(p.shape).clone()}
+            if self.state_bits == 8:
+                state[idx].update(exp_avg_scale=self.exp_avg_scale[run:run + runs].clone(), exp_avg_sq_scale=self.exp_avg_sq_scale[run:run + runs].clone())
+        groups = [{'lr': self.lr * s, 'lr_scale': s, 'betas': tuple(self.betas), 'eps': self.eps, 'weight_decay': self.wd if w is None else w,
+                   'amsgrad': False, 'maximize': False, 'state_bits': self.state_bits, 'seed': self.seed,
+                   'params': sorted(idx for idx, j, _, _, _ in self._slots() if self.group_of[j] == i)} for i, (s, w) in enumerate(self.groups)]
+        return {'state': dict(sorted(state.items())), 'param_groups': groups, 'lr': self.lr, 'weight_decay': self.wd}
+
+    def load_state_dict(self, sd):
+        group = sd['param_groups'][0]
+        if group.get('amsgrad') or group.get('maximize'):
+            raise ValueError('AdamW.load_state_dict: amsgrad and maximize are not built')
+        if int(group.get('state_bits', 32)) != self.state_bits:
+            raise ValueError(f'AdamW.load_state_dict: moments in {group.get("state_bits", 32)} bits, this optimizer holds {self.state_bits}')
+        if 'lr' in sd:
+            self.lr, self.wd = float(sd['lr']), float(sd['weight_decay'])
+        elif len(sd['param_groups']) == 1:                     # a torch.optim.AdamW checkpoint
+            self.lr, self.wd = float(group['lr']), float(group['weight_decay'])
+        self.betas, self.eps, self.seed = tuple(group['betas']), float(group['eps']), int(group.get('seed', self.seed))
+        steps = set()
+        with torch.no_grad():
+            for idx, _, p, run, runs in self._slots():
+                st = sd['state'].get(idx, sd['state'].get(str(idx)))
+                o, n = run * ops.ADAMW_RUN, p.numel()
+                pairs = [(self.exp_avg[o:o + n], 'exp_avg', p.shape), (self.exp_avg_sq[o:o + n], 'exp_avg_sq', p.shape)]
+                if self.state_bits == 8:
+                    pairs += [(self.exp_avg_scale[run:run + runs], 'exp_avg_scale', (runs,)), (self.exp_avg_sq_scale[run:run + runs], 'exp_avg_sq_scale', (runs,))]
+                for dst, name, shape in pairs:
+                    if st is None:                             # a parameter that has not been stepped yet
+                        dst.zero_()
+                        continue
+                    if tuple(st[name].shape) != tuple(shape):
+                        raise ValueError(f'AdamW.load_state_dict: state {idx} has {name} of shape {tuple(st[name].shape)}, expected {tuple(shape)}')
+                    dst.copy_(st[name].reshape(-1))
+                if st is not None:
+                    steps.add(int(st['step']))
+        if len(steps) > 1:
+            raise ValueError(f'AdamW.load_state_dict: parameters at different steps {sorted(steps)}; one step count is kept')
+        self.t = steps.pop() if steps else 0
+        if self._lr_dev is not None:
+            self.push_lr()
 
 
 class OneCycleLR:

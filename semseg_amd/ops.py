@@ -1736,3 +1736,124 @@ def droppath_keep(u, keep_prob):
     out = torch.empty(u.numel(), dtype=torch.float32, device=u.device)
     check(lib().ss_droppath_keep(dt(u), _p(u), float(keep_prob), _p(out), u.numel(), _stream()))
     return out
+
+
+# ---------------------------------------------------------------------------------- residual update between two norms
+_NORM = {'none': 0, None: 0, 'layer': 1, 'rms': 2}
+_GATE_ACT = {'none': 0, None: 0, 'sigmoid': 1}
+
+
+def _resnorm_args(x, b, rows_per_sample, gate, gate_act, scale, keep, post, post_w, post_b, pre, pre_w, pre_b, who):
+    """-> rows, C, gate mode (0 none, 1 per sample, 2 per row), the norms' and the gate's codes; everything a kernel relies on is checked"""
+    rows, C, _ = _mat(x, 'x')
+    if rows == 0 or C == 0:
+        raise ValueError(f'{who}: no rows or no channels')
+    if b.shape != x.shape or _mat(b, 'b')[:2] != (rows, C):
+        raise ValueError(f'{who}: x {tuple(x.shape)} and b {tuple(b.shape)} differ')
+    if (x.dtype, b.dtype) not in ((torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.bfloat16)):
+        raise TypeError(f'{who}: stream / branch types must be f32 / f32, bf16 / bf16 or f32 / bf16, got {x.dtype} / {b.dtype}')
+    n = rows_per_sample or rows
+    if n < 0 or rows % n:
+        raise ValueError(f'{who}: {rows} rows are not whole samples of {n}')
+    samples, mode = rows // n, 0
+    if gate is not None:
+        if gate.dtype != b.dtype or gate.shape[1:] != (C,) or _mat(gate, 'gate')[0] not in (samples, rows):
+            raise ValueError(f'{who}: gate must be {b.dtype} [{samples}, {C}] or [{rows}, {C}], got {gate.dtype} {tuple(gate.shape)}')
+        mode = 2 if gate.shape[0] == rows else 1
+    try:
+        kinds = _NORM[post], _NORM[pre], _GATE_ACT[gate_act]
+    except KeyError as e:
+        raise ValueError(f'{who}: unknown norm or gate activation {e}') from None
+    for kind, w, bias, name in ((kinds[0], post_w, post_b, 'post'), (kinds[1], pre_w, pre_b, 'pre')):
+        if (kind != 0) != (w is not None) or (bias is not None and kind != 1):
+            raise ValueError(f"{who}: {name}: 'layer' takes a weight and optionally a bias, 'rms' a weight, 'none' neither")
+        _f32(w, name + '_weight', C), _f32(bias, name + '_bias', C)
+    _f32(scale, 'scale', C), _f32(keep, 'keep', samples)
+    for t in (b, gate, scale, keep, post_w, post_b, pre_w, pre_b):
+        if t is not None and t.device != x.device:
+            raise ValueError(f'{who}: tensors on {x.device} and {t.device}')
+    return rows, C, n, mode, kinds
+
+
+def resnorm_fwd(x, b, rows_per_sample=0, gate=None, gate_act='none', scale=None, keep=None, alpha=1.0, post='none', post_w=None, post_b=None,
+                pre='none', pre_w=None, pre_b=None, eps=1e-6, want_stats=True):
+    """n = post(b); h = alpha x + keep scale act(gate) n; y = pre(h) on [rows, C] (row strides allowed) -> h, y (None without a norm),
+    stats fp32 [rows, 4] for resnorm_bwd (None unless wanted).  gate: [samples, C] or [rows, C]; keep: fp32 [samples]; rows_per_sample 0:
+    all rows are one sample."""
+    dev = _dev(x)
+    rows, C, n, mode, (post, pre, act) = _resnorm_args(x, b, rows_per_sample, gate, gate_act, scale, keep, post, post_w, post_b, pre, pre_w, pre_b,
+                                                       'resnorm_fwd')
+    with torch.cuda.device(dev):
+        h = torch.empty((rows, C), dtype=x.dtype, device=dev)
+        y = torch.empty((rows, C), dtype=b.dtype, device=dev) if pre else None
+        stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if want_stats else None
+        check(lib().ss_resnorm_fwd(dt(x), dt(b), _p(x), x.stride(0), _p(b), b.stride(0), _p(gate), gate.stride(0) if mode else 0, mode, act, _p(scale),
+                                   _p(keep), alpha, post, _p(post_w), _p(post_b), pre, _p(pre_w), _p(pre_b), eps, _p(h), _p(y), _p(stats), rows, n, C,
+                                   _stream()))
+    return h, y, stats
+
+
+def resnorm_bwd(dh, dy, h, b, stats, rows_per_sample=0, gate=None, gate_act='none', scale=None, keep=None, alpha=1.0, post='none', post_w=None,
+                post_b=None, pre='none', pre_w=None):
+    """Gradients of resnorm_fwd from dh and dy (either may be None) -> dx, db, dgate (None without a gate) and a dict of the fp32 vectors'
+    ('pre_w', 'pre_b', 'post_w', 'post_b', 'scale': those that exist; a LayerNorm's bias always)."""
+    dev = _dev(h)
+    rows, C, n, mode, (post_k, pre_k, act) = _resnorm_args(h, b, rows_per_sample, gate, gate_act, scale, keep, post, post_w, post_b, pre, pre_w, None,
+                                                           'resnorm_bwd')
+    for g, like, name in ((dh, h, 'dh'), (dy, b, 'dy')):
+        if g is not None and (g.shape != h.shape or g.dtype != like.dtype or g.device != dev or _mat(g, name)[1] != C):
+            raise ValueError(f'resnorm_bwd: {name} must be {like.dtype} {tuple(h.shape)} on {dev}')
+    if (dh is None and dy is None) or (dy is not None and not pre_k):
+        raise ValueError('resnorm_bwd: give dh or dy, and dy only with a norm behind h')
+    _f32(stats, 'stats', rows * 4)
+    names = [k for k, there in (('pre_w', pre_k), ('pre_b', pre_k == 1), ('post_w', post_k), ('post_b', post_k == 1), ('scale', scale is not None)) if there]
+    with torch.cuda.device(dev):
+        dx = torch.empty((rows, C), dtype=h.dtype, device=dev)
+        db = torch.empty((rows, C), dtype=b.dtype, device=dev)
+        dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if mode else None
+        dvec = torch.empty((len(names), C), dtype=torch.float32, device=dev)
+        # partial sums from the allocator, not from the shared workspace: two captured graphs may replay side by side
+        ws = torch.empty(lib().ss_resnorm_bwd_workspace(rows, n, C, post_k, pre_k, mode, int(scale is not None)), dtype=torch.uint8, device=dev)
+        check(lib().ss_resnorm_bwd(dt(h), dt(b), _p(dh), dh.stride(0) if dh is not None else 0, _p(dy), dy.stride(0) if dy is not None else 0, _p(h),
+                                   h.stride(0), _p(b), b.stride(0), _p(gate), gate.stride(0) if mode else 0, mode, act, _p(scale), _p(keep), alpha,
+                                   post_k, _p(post_w), _p(post_b), pre_k, _p(pre_w), _p(stats), _p(dx), _p(db), _p(dgate), _p(dvec), rows, n, C, _p(ws),
+                                   ws.numel(), _stream()))
+    return dx, db, dgate, dict(zip(names, dvec))
+
+
+# ---------------------------------------------------------------------------------- many tensors in one launch (optimizer)
+ADAMW_RUN = 256
+
+
+class TensorPlan:
+    """How ss_multi_sqnorm / ss_adamw_step cut a list of tensors into chunks of one workgroup each: sizes only, no addresses.  ``numels``:
+    elements of the tensors; ``groups``: parameter group of each; ``offsets``: given, all tensors lie in ONE buffer at these elements and the
+    launch takes one address.  Each tensor has whole runs of 256 elements in the state, in list order: ``first_run`` of each, ``runs`` of all."""
+
+    def __init__(self, numels, device, groups=None, offsets=None):
+        import ctypes
+        import numpy as np
+        numels = [int(n) for n in numels]
+        groups = [0] * len(numels) if groups is None else list(groups)
+        total = sum(numels)
+        # about eight workgroups a CU where there is that much; 1024 elements (four a thread) at least
+        chunk = 1024
+        while chunk < 8192 and total > chunk * 2048:
+            chunk *= 2
+        rows, first, self.first_run, run = [], [0], [], 0
+        for i, n in enumerate(numels):
+            self.first_run.append(run)
+            base = offsets[i] if offsets is not None else 0
+            for at in range(0, n, chunk):
+                k = min(chunk, n - at)
+                rows.append((base + at, k | (run + at // ADAMW_RUN) << 32, (0 if offsets is not None else i) | groups[i] << 32, 0))
+            run += (n + ADAMW_RUN - 1) // ADAMW_RUN
+            first.append(len(rows))
+        if run >= 1 << 31:
+            raise ValueError('TensorPlan: too many elements')
+        self.runs, self.chunks = run, len(rows)
+        self.count = 1 if offsets is not None else len(numels)
+        first = [0, len(rows)] if offsets is not None else first
+        self.first_chunk = (ctypes.c_int64 * len(first))(*first)
+        self.table = torch.from_numpy(np.array(rows, dtype=np.int64).reshape(-1, 4)).to(device)
+        self.pointers = ctypes.c_void_p * max(self.count, 1)

@@ -1,0 +1,325 @@
+"""Residual update between two norms (ss_resnorm_fwd / _bwd, semseg_amd/resnorm.py) against its 64-bit restatement.
+
+Tolerance of a value: half a step of its type relative to it, plus K 2^-24 times the sum of the absolute values of its terms (the oracle's
+``mag``), a rounding in 32 bits each.  Element-wise values go through at most 20 roundings in a row, two of them of row sums in 32 bits with
+64 terms a lane and join: K = 64.  Column sums add up to 256 rows in a register before they are joined over at most 1024 workgroups in
+chains of 32 and 32: 256 + 64 + 20 roundings, K = 384.  The sigmoid adds v_exp_f32 of an argument scaled in 32 bits: |v| roundings,
+|v| < 16 here, inside both."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+HALF = {torch.float32: U, torch.bfloat16: 2.0 ** -8}
+
+
+def close(got, want, column=False):
+    value, mag = want
+    g = got.detach().double().cpu().reshape(value.shape)
+    tol = HALF[got.dtype] * value.abs() + (384 if column else 64) * U * mag + 1e-38
+    bad = ~((g - value).abs() <= tol)
+    assert not bad.any(), f'{int(bad.sum())} of {bad.numel()} off, worst {float(((g - value).abs() / tol).max()):.3g} x the tolerance'
+
+
+def make(rows, C, stream, branch, seed, *, samples=1, post='none', pre='none', gate='none', act='none', scale=True, keep=False, alpha=1.0, bias=True,
+         offset=0.0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s, dt=torch.float32, m=0.0, k=1.0: (torch.randn(*s, generator=g) * k + m).to(dt)  # noqa: E731
+    t = {'x': r(rows, C, dt=stream, k=2.0, m=offset), 'b': r(rows, C, dt=branch, m=offset - 0.2),
+         'gate': None if gate == 'none' else r(samples if gate == 'sample' else rows, C, dt=branch), 'scale': r(C, k=0.3, m=0.2) if scale else None,
+         'keep': (torch.rand(samples, generator=g) < 0.7).float() / 0.7 if keep else None}
+    for k, kind in (('post', post), ('pre', pre)):
+        t[k + '_w'] = r(C, k=0.3, m=1.0) if kind != 'none' else None
+        t[k + '_b'] = r(C, k=0.3) if kind == 'layer' and bias else None
+    meta = dict(rows_per_sample=rows // samples, gate_act=act, alpha=alpha, post=post, pre=pre)
+    return t, meta, r(rows, C, dt=stream), r(rows, C, dt=branch)
+
+
+def run_and_check(t, meta, dh, dy, eps=1e-6):
+    from semseg_amd import ops
+    from oracle.resnorm import resnorm as oracle
+    d = {k: None if v is None else v.cuda() for k, v in t.items()}
+    fwd = {k: v for k, v in d.items()}
+    h, y, stats = ops.resnorm_fwd(**fwd, **meta, eps=eps)
+    h2, y2, none = ops.resnorm_fwd(**fwd, **meta, eps=eps, want_stats=False)
+    assert torch.equal(h, h2) and none is None and (y is None or torch.equal(y, y2))
+    if meta['pre'] == 'none':
+        dy = None
+    want = oracle(t['x'], t['b'], h.cpu(), dh, dy, eps=eps, **{k: v for k, v in t.items() if k not in 'xb'}, **meta)
+    close(h, want['h'])
+    if y is not None:
+        close(y, want['y'])
+    back = {k: v for k, v in d.items() if k not in ('x', 'b', 'pre_b')}
+    dx, db, dg, G = ops.resnorm_bwd(None if dh is None else dh.cuda(), None if dy is None else dy.cuda(), h, d['b'], stats, **back, **meta)
+    close(dx, want['x']), close(db, want['b'])
+    if dg is not None:
+        close(dg, want['gate'], column=dg.shape[0] != dx.shape[0])
+    assert set(G) == {k for k in ('pre_w', 'pre_b', 'post_w', 'post_b', 'scale') if k in want}
+    for k, v in G.items():
+        close(v, want[k], column=True)
+    return h, y, (dx, db, dg, G)
+
+
+F, H = torch.float32, torch.bfloat16
+TYPES = [(F, F), (H, H), (F, H)]
+
+
+@pytest.mark.parametrize('types', TYPES)
+@pytest.mark.parametrize('rows,C', [(1, 1), (1, 8), (3, 7), (5, 64), (130, 97), (37, 511), (66, 512), (9, 513), (11, 1000), (4, 1024), (6, 1025), (3, 2048),
+                                    (5, 2049), (2, 4095), (7, 4096)])
+def test_widths_both_norms(rows, C, types):
+    run_and_check(*make(rows, C, *types, seed=rows * 7 + C, post='layer', pre='layer', gate='row'))
+
+
+@pytest.mark.parametrize('types', TYPES)
+@pytest.mark.parametrize('pre', ['none', 'layer', 'rms'])
+@pytest.mark.parametrize('post', ['none', 'layer', 'rms'])
+@pytest.mark.parametrize('gate,act', [('none', 'none'), ('sample', 'none'), ('sample', 'sigmoid'), ('row', 'none'), ('row', 'sigmoid')])
+def test_every_form(types, post, pre, gate, act):
+    for i, (rows, C, samples, scale, keep, alpha) in enumerate([(60, 40, 4, True, True, 1.0), (21, 33, 3, False, False, 0.75), (14, 640, 7, True, False, -1.5)]):
+        run_and_check(*make(rows, C, *types, seed=i, samples=samples, post=post, pre=pre, gate=gate, act=act, scale=scale, keep=keep, alpha=alpha, bias=i != 1))
+
+
+@pytest.mark.parametrize('rows,C,samples', [(20000, 64, 4), (30001, 8, 1), (4097, 320, 17), (600, 1500, 3), (5000, 24, 5000), (3000, 768, 1500)])
+def test_many_rows(rows, C, samples):
+    """more rows than one step of all workgroups; samples of many rows, of two, of one; several units to a workgroup"""
+    run_and_check(*make(rows, C, H, H, seed=C, samples=samples, post='rms', pre='layer', gate='sample', keep=True))
+
+
+def test_sums_do_not_cancel_far_from_zero():
+    """rows around 1000 with deviation 1: a variance from 32-bit sums of squares would have no digit left"""
+    run_and_check(*make(50, 768, F, F, seed=3, post='layer', pre='layer', offset=1000.0))
+
+
+@pytest.mark.parametrize('which', ['dh', 'dy'])
+def test_one_gradient_alone(which):
+    t, meta, dh, dy = make(33, 72, H, H, seed=5, post='layer', pre='rms')
+    run_and_check(t, meta, dh if which == 'dh' else None, dy if which == 'dy' else None)
+
+
+def test_constant_rows_and_zero_rows():
+    """no deviation at all: 1 / sqrt(eps), finite everywhere"""
+    t, meta, dh, dy = make(6, 40, F, F, seed=1, post='layer', pre='layer', scale=False)
+    t['b'][:3], t['x'][:3] = 0.0, 0.0
+    t['b'][3:] = 2.5
+    run_and_check(t, meta, dh, dy)
+
+
+def test_rows_with_nan_or_infinity_stay_alone():
+    from semseg_amd import ops
+    t, meta, _, _ = make(40, 48, H, H, seed=2, post='rms', pre='layer')
+    d = {k: None if v is None else v.cuda() for k, v in t.items()}
+    h, y, _ = ops.resnorm_fwd(**d, **meta)
+    d['b'][7, 3], d['b'][21, 5] = float('nan'), float('inf')
+    h2, y2, _ = ops.resnorm_fwd(**d, **meta)
+    ok = torch.ones(40, dtype=torch.bool)
+    ok[[7, 21]] = False
+    assert torch.equal(h[ok.cuda()], h2[ok.cuda()]) and torch.equal(y[ok.cuda()], y2[ok.cuda()])
+    assert y2[7].isnan().all() and y2[21].isnan().all()
+
+
+@pytest.mark.parametrize('types', TYPES)
+@pytest.mark.parametrize('C', [64, 97, 640])
+def test_strided_and_unaligned_rows(types, C):
+    """slices of wider buffers that start anywhere, rows repeated with stride 0: same bits as from dense rows"""
+    from semseg_amd import ops
+    rows = 50
+    t, meta, dh, dy = make(rows, C, *types, seed=C, samples=5, post='layer', pre='rms', gate='sample', act='none', keep=True)
+    d = {k: None if v is None else v.cuda() for k, v in t.items()}
+
+    def inside(v, lead):
+        wide = torch.full((v.shape[0], v.shape[1] + lead + 3), float('nan'), dtype=v.dtype, device='cuda')
+        wide[:, lead:lead + v.shape[1]] = v
+        return wide[:, lead:lead + v.shape[1]]
+    s = dict(d, x=inside(d['x'], 1), b=inside(d['b'], 3), gate=inside(d['gate'], 5))
+    h, y, st = ops.resnorm_fwd(**d, **meta)
+    h2, y2, st2 = ops.resnorm_fwd(**s, **meta)
+    assert torch.equal(h, h2) and torch.equal(y, y2) and torch.equal(st, st2)
+    back = lambda q: {k: v for k, v in q.items() if k not in ('x', 'b', 'pre_b')}  # noqa: E731
+    a = ops.resnorm_bwd(dh.cuda(), dy.cuda(), h, d['b'], st, **back(d), **meta)
+    b = ops.resnorm_bwd(inside(dh.cuda(), 7), inside(dy.cuda(), 1), inside(h, 2), s['b'], st, **back(s), **meta)
+    assert all(torch.equal(p, q) for p, q in zip(a[:3], b[:3])) and all(torch.equal(a[3][k], b[3][k]) for k in a[3])
+    one = d['x'][:1]
+    h3, _, _ = ops.resnorm_fwd(**dict(d, x=one.expand(rows, C)), **meta)
+    h4, _, _ = ops.resnorm_fwd(**dict(d, x=one.expand(rows, C).contiguous()), **meta)
+    assert torch.equal(h3, h4)
+
+
+@pytest.mark.parametrize('C,dtype', [(64, H), (97, F), (4096, H)])
+def test_same_bits_every_time_and_for_every_split(C, dtype):
+    """no atomics: a call repeats itself; and a row's outputs do not depend on how many rows stand beside it"""
+    from semseg_amd import ops
+    t, meta, dh, dy = make(257, C, dtype, dtype, seed=9, post='layer', pre='layer', gate='row')
+    d = {k: None if v is None else v.cuda() for k, v in t.items()}
+    h, y, st = ops.resnorm_fwd(**d, **meta)
+    back = {k: v for k, v in d.items() if k not in ('x', 'b', 'pre_b')}
+    a = ops.resnorm_bwd(dh.cuda(), dy.cuda(), h, d['b'], st, **back, **meta)
+    b = ops.resnorm_bwd(dh.cuda(), dy.cuda(), h, d['b'], st, **back, **meta)
+    assert all(torch.equal(p, q) for p, q in zip(a[:3], b[:3])) and all(torch.equal(a[3][k], b[3][k]) for k in a[3])
+    one = {k: v if v is None or v.dim() == 1 else v[100:101] for k, v in d.items()}
+    h1, y1, _ = ops.resnorm_fwd(**one, **dict(meta, rows_per_sample=1))
+    assert torch.equal(h1, h[100:101]) and torch.equal(y1, y[100:101])
+
+
+# ---------------------------------------------------------------------------------- through autograd and the module
+def _leaves(t):
+    return {k: v.cuda().requires_grad_() if k != 'keep' else v.cuda() for k, v in t.items() if v is not None}
+
+
+@pytest.mark.parametrize('shape', [(4, 15, 40), (2, 3, 5, 24), (30, 40)])
+def test_function_gradients_and_shapes(shape):
+    from semseg_amd import ops
+    from semseg_amd.resnorm import gated_residual_norm
+    C, samples = shape[-1], shape[0] if len(shape) > 2 else 1
+    rows = torch.Size(shape[:-1]).numel()
+    t, meta, dh, dy = make(rows, C, F, H, seed=rows, samples=samples, post='rms', pre='layer', gate='sample', act='sigmoid', keep=True)
+    L = _leaves(t)
+    h, y = gated_residual_norm(L['x'].view(shape), L['b'].view(shape), post='rms', post_weight=L['post_w'], gate=L['gate'], gate_act='sigmoid',
+                               scale=L['scale'], keep=L['keep'], pre='layer', pre_weight=L['pre_w'], pre_bias=L['pre_b'])
+    assert h.shape == y.shape == torch.Size(shape) and h.dtype == F and y.dtype == H
+    names = [k for k in L if k != 'keep']
+    got = dict(zip(names, torch.autograd.grad((h, y), [L[k] for k in names], (dh.cuda().view(shape), dy.cuda().view(shape)))))
+    D = {k: v.detach() for k, v in L.items()}
+    h2, y2, st = ops.resnorm_fwd(**D, **meta)
+    assert torch.equal(h.detach().view(rows, C), h2) and torch.equal(y.detach().view(rows, C), y2)
+    dx, db, dg, G = ops.resnorm_bwd(dh.cuda(), dy.cuda(), h2, D['b'], st, **{k: v for k, v in D.items() if k not in ('x', 'b', 'pre_b')}, **meta)
+    for k, v in dict(G, x=dx, b=db, gate=dg).items():
+        assert torch.equal(got[k], v), k
+
+
+def test_gradients_against_differences():
+    """a directional difference of the fp32 operator itself: step 1e-2 along random directions; the third-order term and the rounding of
+    a sum of 400 terms around 1 are below 2e-3 of it"""
+    from semseg_amd.resnorm import gated_residual_norm
+    t, meta, dh, dy = make(10, 40, F, F, seed=4, samples=2, post='layer', pre='rms', gate='sample', act='sigmoid')
+    L = _leaves(t)
+    dh, dy = dh.cuda().view(2, 5, 40), dy.cuda().view(2, 5, 40)
+
+    def f(P):
+        h, y = gated_residual_norm(P['x'].view(2, 5, 40), P['b'].view(2, 5, 40), post='layer', post_weight=P['post_w'], post_bias=P['post_b'],
+                                   gate=P['gate'], gate_act='sigmoid', scale=P['scale'], pre='rms', pre_weight=P['pre_w'])
+        return (h.double() * dh).sum() + (y.double() * dy).sum()
+    grads = dict(zip(L, torch.autograd.grad(f(L), list(L.values()))))
+    g = torch.Generator(device='cuda').manual_seed(1)
+    for k, v in L.items():
+        d = torch.randn(v.shape, generator=g, device='cuda')
+        with torch.no_grad():
+            num = (f({**L, k: v + 1e-2 * d}) - f({**L, k: v - 1e-2 * d})) / 2e-2
+        exact = (grads[k].double() * d).sum()
+        assert abs(num - exact) <= 2e-3 * (grads[k].double().abs() * d.abs()).sum(), k
+
+
+def test_broadcast_gradients_unused_outputs_and_no_grad():
+    from semseg_amd.resnorm import GatedResidualNorm
+    torch.manual_seed(0)
+    m = GatedResidualNorm(48, post='rms', pre='layer', layer_scale=0.1).cuda()
+    x, b = torch.randn(2, 7, 48, device='cuda', requires_grad=True), torch.randn(2, 7, 48, device='cuda', requires_grad=True)
+    h, y = m(x, b)
+    y.sum().backward()                                        # a gradient with stride 0 everywhere, none for h
+    gx = x.grad.clone()
+    x.grad = None
+    h, y = m(x, b)
+    torch.autograd.backward([y], [torch.ones(2, 7, 48, device='cuda')])
+    assert torch.equal(gx, x.grad)
+    h, y = m(x, b)
+    h.mean().backward()                                       # h alone: the norm behind it gets zero gradients, not garbage
+    assert m.pre_weight.grad is not None and torch.isfinite(m.pre_weight.grad).all()
+    only = GatedResidualNorm(48, pre='none').cuda()
+    h, y = only(x, b)
+    assert y is None and torch.equal(h.detach(), (x + b).detach())
+    h.sum().backward()
+    with torch.no_grad():
+        h2, _ = m(x, b)
+    assert not h2.requires_grad and h2.grad_fn is None
+    wide = torch.randn(2, 7, 96, device='cuda', requires_grad=True)      # a branch and its gate from one projection, row stride 96
+    bb, gg = wide.chunk(2, -1)
+    g = GatedResidualNorm(48, pre='rms', gate_act='sigmoid').cuda()
+    h, y = g(x, bb, gate=gg)
+    (h.sum() + y.sum()).backward()
+    dense = [t.detach().contiguous().requires_grad_() for t in (bb, gg)]
+    h3, y3 = g(x, dense[0], gate=dense[1])
+    (h3.sum() + y3.sum()).backward()
+    assert torch.equal(h, h3) and torch.equal(wide.grad, torch.cat([dense[0].grad, dense[1].grad], -1))
+
+
+def test_retained_graph_backward_twice():
+    from semseg_amd.resnorm import GatedResidualNorm
+    m = GatedResidualNorm(32, pre='layer', layer_scale=1.0).cuda()
+    x = torch.randn(3, 4, 32, device='cuda', requires_grad=True)
+    h, y = m(x, torch.randn(3, 4, 32, device='cuda'))
+    loss = (h * y).sum()
+    a = torch.autograd.grad(loss, [x, m.scale], retain_graph=True)
+    b = torch.autograd.grad(loss, [x, m.scale])
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_drop_path_draws_like_the_framework():
+    from semseg_amd.resnorm import GatedResidualNorm
+    from semseg_amd.runtime import drop_path_keep
+    m = GatedResidualNorm(16, pre='none', drop_path=0.5).cuda().train()
+    x, b = torch.randn(64, 3, 16, device='cuda'), torch.randn(64, 3, 16, device='cuda')
+    torch.manual_seed(5)
+    h, _ = m(x, b)
+    torch.manual_seed(5)
+    keep = drop_path_keep(64, 0.5, torch.float32, x.device)
+    assert 0 < int((keep > 0).sum()) < 64 and torch.equal(h, x + b * keep[:, None, None])
+    assert torch.equal(m.eval()(x, b)[0], x + b)
+
+
+def test_side_stream_and_graph_replays():
+    """the call runs on the caller's stream; captured, it repeats the eager bits at every replay, with eager work in between"""
+    from semseg_amd import ops
+    t, meta, dh, dy = make(700, 96, H, H, seed=8, samples=7, post='layer', pre='layer', gate='sample', keep=True)
+    d = {k: None if v is None else v.cuda() for k, v in t.items()}
+    dh, dy = dh.cuda(), dy.cuda()
+    back = {k: v for k, v in d.items() if k not in ('x', 'b', 'pre_b')}
+
+    def step():
+        h, y, st = ops.resnorm_fwd(**d, **meta)
+        return (h, y) + ops.resnorm_bwd(dh, dy, h, d['b'], st, **back, **meta)
+    flat = lambda r: list(r[:-1]) + list(r[-1].values())  # noqa: E731
+    want = [v.clone() for v in flat(step())]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        side = flat(step())
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(p, q) for p, q in zip(side, want))
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = flat(step())
+        graphs.append((g, out))
+    x0 = d['x'].clone()
+    for k in range(3):
+        d['x'].copy_(x0 * (k + 1))
+        eager = [v.clone() for v in flat(step())]
+        for g, out in graphs:
+            for v in out:
+                v.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(out, eager)), k
+
+
+def test_python_refusals_on_the_device():
+    from semseg_amd import ops
+    x = torch.randn(6, 8, device='cuda')
+    with pytest.raises(ValueError):
+        ops.resnorm_fwd(x, x, pre='layer', pre_w=torch.ones(8))                  # a weight on the host
+    with pytest.raises(ValueError):
+        ops.resnorm_fwd(x.t(), x.t())                                            # inner stride
+    h, y, st = ops.resnorm_fwd(x, x, pre='rms', pre_w=torch.ones(8, device='cuda'))
+    with pytest.raises(ValueError):
+        ops.resnorm_bwd(None, None, h, x, st, pre='rms', pre_w=torch.ones(8, device='cuda'))
+    with pytest.raises(ValueError):
+        ops.resnorm_bwd(x, x, h, x, st)                                          # dy without a norm behind h
+    with pytest.raises(ValueError):
+        ops.resnorm_bwd(x.bfloat16(), None, h, x, st)
+    with pytest.raises(ValueError):
+        ops.resnorm_bwd(x, None, h, x, st[:3])
+    wide = torch.zeros(2, 5000, device='cuda')
+    with pytest.raises(RuntimeError, match='C=5000'):
+        ops.resnorm_fwd(wide, wide)
