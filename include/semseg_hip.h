@@ -563,10 +563,10 @@ int ss_adabound_step(float* p, const float* g, float* m, float* v, int64_t n, do
 
 /* ---- the residual update between two blocks with a norm on either side of it (LayerScale / gated / sandwich-norm residual blocks; the
  * reference has the plain form x + drop_path(gamma * f(norm(x))), modules/convnext.py:38-51, modules/segformer.py:94-98):
- *   n = post(b);  h = alpha x + keep[s] scale[c] act(gate) n;  y = pre(h)        rows r of sample s = r / rows_per_sample, C <= 4096 channels
+ *   n = post(b);  h = alpha x + keep[s] scale[c] act(gate) n;  y = pre(h)        r < 2^30 rows of sample s = r / rows_per_sample, C <= 4096 channels
  * post, pre: 0 none, 1 LayerNorm (weight, bias may be NULL), 2 RMSNorm (weight); gate_mode: 0 none, 1 one row of C per sample, 2 one per row;
  * act: 0 identity, 1 sigmoid.  x and h have x_dtype, b, gate and y b_dtype: f32 / f32, bf16 / bf16 or f32 / bf16.  x, b, gate (and the
- * backward's dh, dy, h) have unit inner stride and their own row stride, aligned to the element only; h, y, dx, db, dgate are dense.  y is
+ * backward's dh, dy, h) have unit inner stride and their own row stride (below 2^23 elements), aligned to the element only; h, y, dx, db, dgate are dense.  y is
  * computed from h as stored.  scale, keep, the weights and the vectors' gradients are float.  stats [rows][4] (optional in the forward): mean
  * and 1 / deviation of b and of h.  Any width of rows, none of them aligned, is taken.  h may not overlap an input. */
 int ss_resnorm_fwd(int x_dtype, int b_dtype, const void* x, int64_t ldx, const void* b, int64_t ldb, const void* gate, int64_t ldg, int gate_mode,

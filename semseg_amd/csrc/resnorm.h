@@ -1,0 +1,153 @@
+// What the forward and the backward of the residual update between two norms share: eight channels of a row, row sums, the vectors in LDS.
+#pragma once
+#include "common.h"
+
+// ---------------------------------------------------------------- eight channels of a row
+// Row starts need no alignment beyond the element's (odd widths, odd row strides): global memory takes the access as one.
+struct __attribute__((packed, aligned(2))) Bf8u { bf16x8 v; };
+struct __attribute__((packed, aligned(4))) Fl8u { floatx4 a, b; };
+template <typename T> struct Chunk;
+template <> struct Chunk<bf16> {
+    bf16x8 v;
+    __device__ __forceinline__ void load(const bf16* p) { v = ((const Bf8u*)p)->v; }
+    __device__ __forceinline__ float get(int e) const { return (float)v[e]; }
+    __device__ __forceinline__ void set(int e, float f) { v[e] = (bf16)f; }
+    __device__ __forceinline__ void store(bf16* p) const { ((Bf8u*)p)->v = v; }
+};
+template <> struct Chunk<float> {
+    floatx4 a, b;
+    __device__ __forceinline__ void load(const float* p) { a = ((const Fl8u*)p)->a; b = ((const Fl8u*)p)->b; }
+    __device__ __forceinline__ float get(int e) const { return e < 4 ? a[e & 3] : b[e & 3]; }
+    __device__ __forceinline__ void set(int e, float f) { if (e < 4) a[e & 3] = f; else b[e & 3] = f; }
+    __device__ __forceinline__ void store(float* p) const { ((Fl8u*)p)->a = a; ((Fl8u*)p)->b = b; }
+};
+// The eight channels of a lane: [cb, cb + 8), of which e in [lo, hi) are its own.  At the end of a row whose width is no multiple of eight
+// the last chunk is moved back to end with the row, and a lane past the row's end reads that chunk too and owns nothing: every load is a
+// whole chunk inside the row, without a branch.  (A load under a branch may not have been issued, so a wait for an older one has to
+// wait for everything, and the next row's loads are not in flight any more: ConvNeXt stage 3 backward 101 us against 75.)
+struct Cols { int cb, lo, hi; };
+__device__ __forceinline__ Cols cols_of(int c, int C) {
+    const int n = C - c;
+    Cols r;
+    r.cb = n >= 8 ? c : C >= 8 ? C - 8 : 0;
+    r.lo = n >= 8 ? 0 : n <= 0 ? 8 : C >= 8 ? 8 - n : 0;
+    r.hi = C >= 8 ? 8 : C;
+    return r;
+}
+// compared where it is used: sixteen lane masks kept over a loop do not fit the scalar registers
+__device__ __forceinline__ Cols here(Cols k) { asm volatile("" : "+v"(k.lo), "+v"(k.hi)); return k; }
+// a row of less than eight channels is loaded one by one (every lane of the launch alike)
+template <typename T> __device__ __forceinline__ void load_chunk(Chunk<T>& t, const T* p, int C) {
+    if (C >= 8) t.load(p);
+    else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t.set(e, to_f(p[e < C ? e : C - 1]));
+    }
+}
+template <typename T> __device__ __forceinline__ void store_chunk(const Chunk<T>& t, T* p, const Cols& k) {
+    if (k.lo == 0 && k.hi == 8) { t.store(p); return; }
+    const Cols own = here(k);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) if (e >= own.lo && e < own.hi) p[e] = from_f<T>(t.get(e));
+}
+
+// Address of a lane's element: a row that the whole wave agrees on (64 bits, scalar registers) and the lane's offset from it (32 bits): one
+// vector register a tensor instead of two for every pointer.  The host keeps 64 row strides below 2^32 bytes.
+template <typename T> __device__ __forceinline__ T* at(T* base, int row, int ld, unsigned off) {
+    return (T*)((char*)(base + (int64_t)row * ld) + off * (unsigned)sizeof(T));
+}
+template <typename T> __device__ __forceinline__ const T* at(const void* base, int row, int ld, unsigned off) {
+    return (const T*)((const char*)((const T*)base + (int64_t)row * ld) + off * (unsigned)sizeof(T));
+}
+#define SS_RESNORM_MAX_LD (1LL << 23)
+#define SS_RESNORM_MAX_ROWS (1LL << 30)
+
+// ---------------------------------------------------------------- row sums
+template <int CTRL> __device__ __forceinline__ double dpp_add_d(double v) {
+    const long long u = __builtin_bit_cast(long long, v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)u, CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, 0xf, 0xf, true);
+    return v + __builtin_bit_cast(double, ((long long)hi << 32) | (unsigned)lo);
+}
+__device__ __forceinline__ double dgroup_sum(double v, int lanes) {         // over aligned groups of a power of two of lanes
+    if (lanes >= 2) v = dpp_add_d<0xB1>(v);
+    if (lanes >= 4) v = dpp_add_d<0x4E>(v);
+    if (lanes >= 8) v = dpp_add_d<0x141>(v);
+    if (lanes >= 16) v = dpp_add_d<0x140>(v);
+    for (int o = 16; o < lanes; o <<= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+// Two sums over the lanes of a row.  `sh` has two halves used in turn: a wave may enter the next sum while another still reads this one,
+// but not the one after it.
+template <int WAVES, typename S> __device__ __forceinline__ void row_sum2(S& a, S& b, int lanes, S* sh, int& turn) {
+    if constexpr (sizeof(S) == 8) { a = dgroup_sum(a, lanes); b = dgroup_sum(b, lanes); }
+    else { a = group_sum(a, lanes); b = group_sum(b, lanes); }
+    if constexpr (WAVES == 1) __builtin_amdgcn_sched_barrier(0);            // what follows is not moved up here: it would only take registers
+    if constexpr (WAVES > 1) {
+        S* s = sh + turn * 2 * WAVES;
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0) { s[(threadIdx.x >> 6) * 2] = a; s[(threadIdx.x >> 6) * 2 + 1] = b; }
+        __syncthreads();
+        a = s[0]; b = s[1];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) { a += s[w * 2]; b += s[w * 2 + 1]; }
+    }
+}
+// 1 / sqrt(x) from v_rsq_f64 (about 26 bits) and one Newton step
+__device__ __forceinline__ double rsqrt_d(double x) {
+    const double y = __builtin_amdgcn_rsq(x);
+    return y * fma(-0.5 * x * y, y, 1.5);
+}
+template <int WAVES> __device__ __forceinline__ void row_stats(double s, double q, int kind, double inv_c, double eps, int lanes, double* sh, int& turn, float& mu, float& r) {
+    row_sum2<WAVES>(s, q, lanes, sh, turn);
+    const double m = kind == 1 ? s * inv_c : 0.0;
+    double var = fma(-m, m, q * inv_c);
+    var = var > 0.0 ? var : (var < 0.0 ? 0.0 : var);                        // NaN stays
+    mu = (float)m; r = (float)rsqrt_d(var + eps);
+}
+__device__ __forceinline__ float sigmoid_f(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
+
+// ---------------------------------------------------------------- the vectors (weights, biases, scale) in LDS
+// One row of `chunks` chunks per vector, the two halves of a chunk apart: lanes read 16 bytes each, 16 bytes apart.  Where a chunk's channel
+// is not the lane's own the vectors are ZERO.
+__device__ __forceinline__ float vec_value(const float* p, float otherwise, int C, int i) {
+    const Cols k = cols_of(i & ~7, C);
+    const int e = i & 7;
+    return e < k.lo || e >= k.hi ? 0.f : p ? p[k.cb + e] : otherwise;
+}
+__device__ __forceinline__ void stage_vec(float* sh, const float* p, float otherwise, int C, int chunks, int threads) {
+    for (int i = threadIdx.x; i < chunks * 8; i += threads) sh[((i >> 2) & 1) * chunks * 4 + (i >> 3) * 4 + (i & 3)] = vec_value(p, otherwise, C, i);
+}
+// the same for a thread that owns its columns
+__device__ __forceinline__ void load_vec(float (&v)[8], const float* p, float otherwise, const Cols& k) {
+    if (p) {
+        Chunk<float> t;
+        t.load(p + k.cb);                                                    // C > 8 here
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < k.lo ? 0.f : t.get(e);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < k.lo ? 0.f : otherwise;
+    }
+}
+__device__ __forceinline__ void vec_chunk(float (&v)[8], const float* sh, int chunk, int chunks) {
+    const floatx4 a = *(const floatx4*)(sh + chunk * 4), b = *(const floatx4*)(sh + chunks * 4 + chunk * 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+}
+
+// ---------------------------------------------------------------- C ABI: what both entries check
+#define SS_RESNORM_MAX_C 4096
+static inline int resnorm_check(const char* who, int x_dtype, int b_dtype, int64_t rows, int64_t rows_per_sample, int C, int post, int pre, int gate_mode,
+                         int act, const void* gate, const float* post_w, const float* post_b, const float* pre_w, const float* pre_b, bool biases) {
+    SS_CHECK((x_dtype == SS_F32 && (b_dtype == SS_F32 || b_dtype == SS_BF16)) || (x_dtype == SS_BF16 && b_dtype == SS_BF16),
+             "%s: stream / branch types must be f32 / f32, bf16 / bf16 or f32 / bf16, got codes %d / %d", who, x_dtype, b_dtype);
+    SS_CHECK(rows > 0 && rows < SS_RESNORM_MAX_ROWS && rows_per_sample > 0 && rows % rows_per_sample == 0, "%s: bad row counts (%lld, %lld a sample)", who,
+             (long long)rows, (long long)rows_per_sample);
+    SS_CHECK(C > 0 && C <= SS_RESNORM_MAX_C, "%s: C=%d must be 1 to %d", who, C, SS_RESNORM_MAX_C);
+    SS_CHECK(post >= 0 && post <= 2 && pre >= 0 && pre <= 2 && gate_mode >= 0 && gate_mode <= 2 && act >= 0 && act <= 1, "%s: bad codes", who);
+    SS_CHECK((gate_mode != 0) == (gate != nullptr), "%s: a gate and its layout go together", who);
+    SS_CHECK((!post || post_w) && (!pre || pre_w), "%s: a norm needs its weight", who);
+    SS_CHECK(!biases || ((post == 1 || !post_b) && (pre == 1 || !pre_b)), "%s: only LayerNorm takes a bias", who);
+    return 0;
+}
+

@@ -1743,6 +1743,25 @@ _NORM = {'none': 0, None: 0, 'layer': 1, 'rms': 2}
 _GATE_ACT = {'none': 0, None: 0, 'sigmoid': 1}
 
 
+_STREAMS = {(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.bfloat16)}
+
+
+def _resnorm_vectors(C, samples, device, gate_act, scale, keep, post, post_w, post_b, pre, pre_w, pre_b, who):
+    """-> codes of the norms and of the gate's activation"""
+    try:
+        kinds = _NORM[post], _NORM[pre], _GATE_ACT[gate_act]
+    except KeyError as e:
+        raise ValueError(f'{who}: unknown norm or gate activation {e}') from None
+    if (kinds[0] != 0) != (post_w is not None) or (post_b is not None and kinds[0] != 1) or (kinds[1] != 0) != (pre_w is not None) or \
+            (pre_b is not None and kinds[1] != 1):
+        raise ValueError(f"{who}: 'layer' takes a weight and optionally a bias, 'rms' a weight, 'none' neither")
+    for t, name, n in ((post_w, 'post_weight', C), (post_b, 'post_bias', C), (pre_w, 'pre_weight', C), (pre_b, 'pre_bias', C), (scale, 'scale', C),
+                       (keep, 'keep', samples)):
+        if t is not None and (t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous() or t.device != device):
+            raise ValueError(f'{who}: {name} must be contiguous float32 of {n} elements on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}')
+    return kinds
+
+
 def _resnorm_args(x, b, rows_per_sample, gate, gate_act, scale, keep, post, post_w, post_b, pre, pre_w, pre_b, who):
     """-> rows, C, gate mode (0 none, 1 per sample, 2 per row), the norms' and the gate's codes; everything a kernel relies on is checked"""
     rows, C, _ = _mat(x, 'x')
@@ -1750,7 +1769,7 @@ def _resnorm_args(x, b, rows_per_sample, gate, gate_act, scale, keep, post, post
         raise ValueError(f'{who}: no rows or no channels')
     if b.shape != x.shape or _mat(b, 'b')[:2] != (rows, C):
         raise ValueError(f'{who}: x {tuple(x.shape)} and b {tuple(b.shape)} differ')
-    if (x.dtype, b.dtype) not in ((torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.bfloat16)):
+    if (x.dtype, b.dtype) not in _STREAMS:
         raise TypeError(f'{who}: stream / branch types must be f32 / f32, bf16 / bf16 or f32 / bf16, got {x.dtype} / {b.dtype}')
     n = rows_per_sample or rows
     if n < 0 or rows % n:
@@ -1760,19 +1779,64 @@ def _resnorm_args(x, b, rows_per_sample, gate, gate_act, scale, keep, post, post
         if gate.dtype != b.dtype or gate.shape[1:] != (C,) or _mat(gate, 'gate')[0] not in (samples, rows):
             raise ValueError(f'{who}: gate must be {b.dtype} [{samples}, {C}] or [{rows}, {C}], got {gate.dtype} {tuple(gate.shape)}')
         mode = 2 if gate.shape[0] == rows else 1
-    try:
-        kinds = _NORM[post], _NORM[pre], _GATE_ACT[gate_act]
-    except KeyError as e:
-        raise ValueError(f'{who}: unknown norm or gate activation {e}') from None
-    for kind, w, bias, name in ((kinds[0], post_w, post_b, 'post'), (kinds[1], pre_w, pre_b, 'pre')):
-        if (kind != 0) != (w is not None) or (bias is not None and kind != 1):
-            raise ValueError(f"{who}: {name}: 'layer' takes a weight and optionally a bias, 'rms' a weight, 'none' neither")
-        _f32(w, name + '_weight', C), _f32(bias, name + '_bias', C)
-    _f32(scale, 'scale', C), _f32(keep, 'keep', samples)
-    for t in (b, gate, scale, keep, post_w, post_b, pre_w, pre_b):
+    for t in (b, gate):
         if t is not None and t.device != x.device:
             raise ValueError(f'{who}: tensors on {x.device} and {t.device}')
-    return rows, C, n, mode, kinds
+    return rows, C, n, mode, _resnorm_vectors(C, samples, x.device, gate_act, scale, keep, post, post_w, post_b, pre, pre_w, pre_b, who)
+
+
+class _DeviceGuard:
+    """``torch.cuda.device`` where the device is not the current one, nothing (0.1 us) where it is"""
+    __slots__ = ('index', 'ctx')
+
+    def __init__(self, device):
+        self.index, self.ctx = device.index, None
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self.index:
+            self.ctx = torch.cuda.device(self.index)
+            self.ctx.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self.index)  # what torch.cuda.current_stream(index).cuda_stream is, without the object
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+def _resnorm_launch_fwd(x, ldx, b, ldb, gate, ldg, mode, act, scale, keep, alpha, post, post_w, post_b, pre, pre_w, pre_b, eps, want_stats, rows, n, C, shape):
+    """checked arguments -> h, y of `shape`, stats"""
+    dev = x.device
+    with _DeviceGuard(dev) as stream:
+        h = torch.empty(shape, dtype=x.dtype, device=dev)
+        y = torch.empty(shape, dtype=b.dtype, device=dev) if pre else None
+        stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if want_stats else None
+        check(lib().ss_resnorm_fwd(_DT[x.dtype], _DT[b.dtype], x.data_ptr(), ldx, b.data_ptr(), ldb, _p(gate), ldg, mode, act, _p(scale), _p(keep), alpha, post,
+                                   _p(post_w), _p(post_b), pre, _p(pre_w), _p(pre_b), eps, h.data_ptr(), _p(y), _p(stats), rows, n, C, stream))
+    return h, y, stats
+
+
+def _resnorm_launch_bwd(dh, lddh, dy, lddy, h, ldh, b, ldb, stats, gate, ldg, mode, act, scale, keep, alpha, post, post_w, post_b, pre, pre_w, rows, n, C,
+                        shape):
+    """checked arguments -> dx, db of `shape`, dgate like gate, the vectors' gradients fp32 [slots, C]"""
+    dev = h.device
+    slots = (pre != 0) + (pre == 1) + (post != 0) + (post == 1) + (scale is not None)
+    with _DeviceGuard(dev) as stream:
+        dx = torch.empty(shape, dtype=h.dtype, device=dev)
+        db = torch.empty(shape, dtype=b.dtype, device=dev)
+        dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if mode else None
+        # the vectors' gradients and, behind them, the partial sums: from the allocator, not from the shared workspace, since two captured
+        # graphs may replay side by side
+        need = lib().ss_resnorm_bwd_workspace(rows, n, C, post, pre, mode, int(scale is not None))
+        buf = torch.empty(slots * C + need // 4, dtype=torch.float32, device=dev)
+        base = buf.data_ptr()
+        check(lib().ss_resnorm_bwd(_DT[h.dtype], _DT[b.dtype], _p(dh), lddh, _p(dy), lddy, h.data_ptr(), ldh, b.data_ptr(), ldb, _p(gate), ldg, mode, act,
+                                   _p(scale), _p(keep), alpha, post, _p(post_w), _p(post_b), pre, _p(pre_w), stats.data_ptr(), dx.data_ptr(), db.data_ptr(),
+                                   _p(dgate), base, rows, n, C, base + slots * C * 4, need, stream))
+    return dx, db, dgate, buf[:slots * C].view(slots, C) if slots else buf
+
+
+def _resnorm_slots(post, pre, scale):
+    return [k for k, there in (('pre_w', pre), ('pre_b', pre == 1), ('post_w', post), ('post_b', post == 1), ('scale', scale is not None)) if there]
 
 
 def resnorm_fwd(x, b, rows_per_sample=0, gate=None, gate_act='none', scale=None, keep=None, alpha=1.0, post='none', post_w=None, post_b=None,
@@ -1780,17 +1844,11 @@ def resnorm_fwd(x, b, rows_per_sample=0, gate=None, gate_act='none', scale=None,
     """n = post(b); h = alpha x + keep scale act(gate) n; y = pre(h) on [rows, C] (row strides allowed) -> h, y (None without a norm),
     stats fp32 [rows, 4] for resnorm_bwd (None unless wanted).  gate: [samples, C] or [rows, C]; keep: fp32 [samples]; rows_per_sample 0:
     all rows are one sample."""
-    dev = _dev(x)
+    _dev(x)
     rows, C, n, mode, (post, pre, act) = _resnorm_args(x, b, rows_per_sample, gate, gate_act, scale, keep, post, post_w, post_b, pre, pre_w, pre_b,
                                                        'resnorm_fwd')
-    with torch.cuda.device(dev):
-        h = torch.empty((rows, C), dtype=x.dtype, device=dev)
-        y = torch.empty((rows, C), dtype=b.dtype, device=dev) if pre else None
-        stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if want_stats else None
-        check(lib().ss_resnorm_fwd(dt(x), dt(b), _p(x), x.stride(0), _p(b), b.stride(0), _p(gate), gate.stride(0) if mode else 0, mode, act, _p(scale),
-                                   _p(keep), alpha, post, _p(post_w), _p(post_b), pre, _p(pre_w), _p(pre_b), eps, _p(h), _p(y), _p(stats), rows, n, C,
-                                   _stream()))
-    return h, y, stats
+    return _resnorm_launch_fwd(x, x.stride(0), b, b.stride(0), gate, gate.stride(0) if mode else 0, mode, act, scale, keep, alpha, post, post_w, post_b, pre,
+                               pre_w, pre_b, eps, want_stats, rows, n, C, (rows, C))
 
 
 def resnorm_bwd(dh, dy, h, b, stats, rows_per_sample=0, gate=None, gate_act='none', scale=None, keep=None, alpha=1.0, post='none', post_w=None,
@@ -1806,19 +1864,10 @@ def resnorm_bwd(dh, dy, h, b, stats, rows_per_sample=0, gate=None, gate_act='non
     if (dh is None and dy is None) or (dy is not None and not pre_k):
         raise ValueError('resnorm_bwd: give dh or dy, and dy only with a norm behind h')
     _f32(stats, 'stats', rows * 4)
-    names = [k for k, there in (('pre_w', pre_k), ('pre_b', pre_k == 1), ('post_w', post_k), ('post_b', post_k == 1), ('scale', scale is not None)) if there]
-    with torch.cuda.device(dev):
-        dx = torch.empty((rows, C), dtype=h.dtype, device=dev)
-        db = torch.empty((rows, C), dtype=b.dtype, device=dev)
-        dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if mode else None
-        dvec = torch.empty((len(names), C), dtype=torch.float32, device=dev)
-        # partial sums from the allocator, not from the shared workspace: two captured graphs may replay side by side
-        ws = torch.empty(lib().ss_resnorm_bwd_workspace(rows, n, C, post_k, pre_k, mode, int(scale is not None)), dtype=torch.uint8, device=dev)
-        check(lib().ss_resnorm_bwd(dt(h), dt(b), _p(dh), dh.stride(0) if dh is not None else 0, _p(dy), dy.stride(0) if dy is not None else 0, _p(h),
-                                   h.stride(0), _p(b), b.stride(0), _p(gate), gate.stride(0) if mode else 0, mode, act, _p(scale), _p(keep), alpha,
-                                   post_k, _p(post_w), _p(post_b), pre_k, _p(pre_w), _p(stats), _p(dx), _p(db), _p(dgate), _p(dvec), rows, n, C, _p(ws),
-                                   ws.numel(), _stream()))
-    return dx, db, dgate, dict(zip(names, dvec))
+    dx, db, dgate, dvec = _resnorm_launch_bwd(dh, dh.stride(0) if dh is not None else 0, dy, dy.stride(0) if dy is not None else 0, h, h.stride(0), b,
+                                              b.stride(0), stats, gate, gate.stride(0) if mode else 0, mode, act, scale, keep, alpha, post_k, post_w, post_b,
+                                              pre_k, pre_w, rows, n, C, (rows, C))
+    return dx, db, dgate, dict(zip(_resnorm_slots(post_k, pre_k, scale), dvec))
 
 
 # ---------------------------------------------------------------------------------- many tensors in one launch (optimizer)

@@ -19,37 +19,53 @@ _VECTORS = ('pre_w', 'pre_b', 'post_w', 'post_b', 'scale')
 
 
 def _rows(t, C):
-    """[..., C] -> [rows, C] with unit inner stride; a copy only where the layout asks for one (a broadcast gradient, split strides)"""
-    t = t.reshape(-1, C)
-    return t if t.stride(1) == 1 else t.contiguous().as_strided(t.shape, (C, 1))
+    """[..., C] -> (tensor, elements between rows) with unit inner stride; a view or a copy only where the layout asks for one (a broadcast
+    gradient, split strides)"""
+    if t.is_contiguous():
+        return t, C
+    if t.dim() != 2:
+        t = t.reshape(-1, C)
+    if t.stride(1) != 1:
+        t = t.contiguous()
+        return t, C
+    return t, t.stride(0)
 
 
 class _ResnormFn(GradAwareFunction):
+    """``cfg``: what ``gated_residual_norm`` checked -- rows, rows of a sample, C, gate mode, codes of post, pre and the activation, alpha, eps"""
+
     @staticmethod
-    def forward(ctx, x, b, gate, keep, meta, *vectors):
-        C = x.shape[-1]
-        h, y, stats = ops.resnorm_fwd(_rows(x.detach(), C), _rows(b.detach(), C), gate=None if gate is None else _rows(gate.detach(), C), keep=keep,
-                                      **meta, **dict(zip(_VECTORS, vectors)))
-        h = h.view(x.shape)
-        ctx.meta = {k: v for k, v in meta.items() if k != 'eps'}
+    def forward(ctx, x, b, gate, keep, cfg, *vectors):
+        rows, n, C, mode, post, pre, act, alpha, eps = cfg
+        pre_w, pre_b, post_w, post_b, scale = vectors
+        xs, ldx = _rows(x, C)
+        bs, ldb = _rows(b, C)
+        gs, ldg = _rows(gate, C) if mode else (None, 0)
+        h, y, stats = ops._resnorm_launch_fwd(xs, ldx, bs, ldb, gs, ldg, mode, act, scale, keep, alpha, post, post_w, post_b, pre, pre_w, pre_b, eps, True,
+                                              rows, n, C, x.shape)
+        ctx.cfg = cfg
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(h, b, gate, keep, stats, *vectors)
         expect_grads(ctx, vectors, 5)
-        return h, None if y is None else y.view(x.shape)
+        return h, y
 
     @staticmethod
     def backward(ctx, dh, dy):
-        h, b, gate, keep, stats, *vectors = ctx.saved_tensors
-        need = ctx.needs_input_grad
         if dh is None and dy is None:
-            return (None,) * (5 + len(vectors))
-        C = h.shape[-1]
-        V = {k: v for k, v in zip(_VECTORS, vectors) if k != 'pre_b'}
-        dx, db, dgate, G = ops.resnorm_bwd(None if dh is None else _rows(dh, C), None if dy is None else _rows(dy, C), _rows(h, C), _rows(b, C), stats,
-                                           gate=None if gate is None else _rows(gate, C), keep=keep, **ctx.meta, **V)
-        grads = deliver_grads(vectors, [G[k].view(v.shape) if v is not None and need[5 + i] else None for i, (k, v) in enumerate(zip(_VECTORS, vectors))])
-        return (dx.view(h.shape) if need[0] else None, db.view(b.shape) if need[1] else None,
-                dgate.view(gate.shape) if gate is not None and need[2] else None, None, None, *grads)
+            return (None,) * 10
+        rows, n, C, mode, post, pre, act, alpha, _ = ctx.cfg
+        h, b, gate, keep, stats, *vectors = ctx.saved_tensors
+        _, _, post_w, post_b, scale = vectors
+        need = ctx.needs_input_grad
+        dhs, lddh = (None, 0) if dh is None else _rows(dh, C)
+        dys, lddy = (None, 0) if dy is None else _rows(dy, C)
+        bs, ldb = _rows(b, C)
+        gs, ldg = _rows(gate, C) if mode else (None, 0)
+        dx, db, dgate, dvec = ops._resnorm_launch_bwd(dhs, lddh, dys, lddy, h, C, bs, ldb, stats, gs, ldg, mode, act, scale, keep, alpha, post, post_w, post_b,
+                                                      pre, vectors[0], rows, n, C, h.shape)
+        made = dict(zip(ops._resnorm_slots(post, pre, scale), dvec.unbind(0)))
+        grads = deliver_grads(vectors, [made[k] if v is not None and need[5 + i] else None for i, (k, v) in enumerate(zip(_VECTORS, vectors))])
+        return (dx if need[0] else None, db if need[1] else None, dgate.view(gate.shape) if mode and need[2] else None, None, None, *grads)
 
 
 def gated_residual_norm(x: Tensor, branch: Tensor, *, post='none', post_weight=None, post_bias=None, gate=None, gate_act='none', scale=None, keep=None,
@@ -60,22 +76,38 @@ def gated_residual_norm(x: Tensor, branch: Tensor, *, post='none', post_weight=N
     (weight, optionally bias) or 'rms' (weight).  gate (branch's type): per sample [samples, C] or per element, shaped like x; gate_act:
     'none' or 'sigmoid'.  scale, weights, biases: float32 [C].  keep: float32 [samples].  A sample is an index of x's first dimension (a 2-D
     x is one sample) unless ``samples`` says into how many equal runs of rows x divides.  Differentiable in everything but keep."""
-    if x.dim() < 2 or x.shape != branch.shape:
-        raise ValueError(f'gated_residual_norm: x {tuple(x.shape)} and branch {tuple(branch.shape)} must be alike, [..., C]')
-    C, rows = x.shape[-1], x.numel() // max(x.shape[-1], 1)
+    shape = x.shape
+    if len(shape) < 2 or branch.shape != shape:
+        raise ValueError(f'gated_residual_norm: x {tuple(shape)} and branch {tuple(branch.shape)} must be alike, [..., C]')
+    C, total, device = shape[-1], x.numel(), x.device
+    if total == 0:
+        raise ValueError(f'gated_residual_norm: nothing in x {tuple(shape)}')
+    rows = total // C
     if samples is None:
-        samples = x.shape[0] if x.dim() > 2 else 1
+        samples = shape[0] if len(shape) > 2 else 1
     if samples < 1 or rows % samples:
         raise ValueError(f'gated_residual_norm: {rows} rows do not divide into {samples} samples')
-    if gate is not None and gate.shape != x.shape and gate.shape != (samples, C):
-        raise ValueError(f'gated_residual_norm: gate must be [{samples}, {C}] or like x, got {tuple(gate.shape)}')
-    meta = {'rows_per_sample': rows // samples, 'gate_act': gate_act, 'alpha': float(alpha), 'post': post, 'pre': pre, 'eps': float(eps)}
+    mode = 0
+    if gate is not None:
+        mode = 2 if gate.shape == shape else 1 if gate.shape == (samples, C) else 0
+        if mode == 0 or gate.dtype != branch.dtype:
+            raise ValueError(f'gated_residual_norm: gate must be {branch.dtype} [{samples}, {C}] or like x, got {gate.dtype} {tuple(gate.shape)}')
+    ops._dev(x)
+    if branch.device != device or (mode and gate.device != device):
+        raise ValueError('gated_residual_norm: x, branch and gate must be on one device')
+    if (x.dtype, branch.dtype) not in ops._STREAMS:
+        raise TypeError(f'gated_residual_norm: stream / branch types must be f32 / f32, bf16 / bf16 or f32 / bf16, got {x.dtype} / {branch.dtype}')
+    post_k, pre_k, act = ops._resnorm_vectors(C, samples, device, gate_act, scale, keep, post, post_weight, post_bias, pre, pre_weight, pre_bias,
+                                              'gated_residual_norm')
     vectors = (pre_weight, pre_bias, post_weight, post_bias, scale)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, branch, gate) + vectors):
-        return _ResnormFn.apply(x, branch, gate, keep, meta, *vectors)
-    h, y, _ = ops.resnorm_fwd(_rows(x, C), _rows(branch, C), gate=None if gate is None else _rows(gate, C), keep=keep, want_stats=False, **meta,
-                              **dict(zip(_VECTORS, vectors)))
-    return h.view(x.shape), None if y is None else y.view(x.shape)
+    if torch.is_grad_enabled() and (x.requires_grad or branch.requires_grad or (mode and gate.requires_grad) or
+                                    any(t is not None and t.requires_grad for t in vectors)):
+        return _ResnormFn.apply(x, branch, gate, keep, (rows, rows // samples, C, mode, post_k, pre_k, act, float(alpha), float(eps)), *vectors)
+    xs, ldx = _rows(x, C)
+    bs, ldb = _rows(branch, C)
+    gs, ldg = _rows(gate, C) if mode else (None, 0)
+    return ops._resnorm_launch_fwd(xs, ldx, bs, ldb, gs, ldg, mode, act, scale, keep, alpha, post_k, post_weight, post_bias, pre_k, pre_weight, pre_bias, eps,
+                                   False, rows, rows // samples, C, shape)[:2]
 
 
 class GatedResidualNorm(nn.Module):
