@@ -597,19 +597,25 @@ int ss_resnorm_bwd(int x_dtype, int b_dtype, const void* dh, int64_t lddh, const
  *   makes its run NaN.  The parameter is updated from the moments before they are rounded.
  * lr and weight_decay are HOST arrays of `groups` <= 64 doubles.  `dyn` (device, ss_adamw_dyn_workspace() bytes), when given, holds what
  * ss_adamw_prepare left there and stands in for grad_scale, t, lr, weight_decay and seed. */
-int ss_multi_sqnorm(int dtype, int count, const void* const* grads, const int64_t* first_chunk, const void* plan, double* partial /* [chunks] */,
-                    hipStream_t stream);
+/* sums of squares of all gradients, one double per workgroup: ss_multi_sqnorm_workspace() bytes, in a fixed order */
+int64_t ss_multi_sqnorm_workspace(int count, const int64_t* first_chunk);
+int ss_multi_sqnorm(int dtype, int count, const void* const* grads, const int64_t* first_chunk, const void* plan, double* partial, hipStream_t stream);
 int64_t ss_adamw_dyn_workspace(void);
-/* One workgroup: norm from the partial sums (may be none), clipping coefficient, bias corrections and learning rates into `dyn`.  t_dev, when
+/* One workgroup: norm from the `count` partial sums (may be none), clipping coefficient, bias corrections and learning rates into `dyn`.  t_dev, when
  * given, is the step count on the device: it is advanced by one and used instead of t (a captured graph counts its replays so); lr_dev, when
  * given, is double[groups] on the device and read instead of lr.  max_norm <= 0: no clipping.  skip_nonfinite: with a norm that is infinite or
  * NaN the step count stays and ss_adamw_step changes nothing. */
-int ss_adamw_prepare(const double* partial, int64_t chunks, double max_norm, double grad_scale, double beta1, double beta2, int64_t t,
+int ss_adamw_prepare(const double* partial, int64_t count, double max_norm, double grad_scale, double beta1, double beta2, int64_t t,
                      int64_t* t_dev, int groups, const double* lr, const double* weight_decay, const double* lr_dev, int64_t seed,
                      int skip_nonfinite, float* norm, void* dyn, hipStream_t stream);
 int ss_adamw_step(int p_dtype, int g_dtype, int bits, int count, void* const* params, const void* const* grads, const int64_t* first_chunk,
                   const void* plan, void* m, void* v, float* m_scale, float* v_scale, double beta1, double beta2, double eps, double grad_scale,
                   int64_t t, int groups, const double* lr, const double* weight_decay, int64_t seed, const void* dyn, hipStream_t stream);
+/* the three in one call; without `partial` (ss_multi_sqnorm_workspace() bytes) the norm is not measured */
+int ss_adamw_clip_step(int p_dtype, int g_dtype, int bits, int count, void* const* params, const void* const* grads, const int64_t* first_chunk,
+                       const void* plan, void* m, void* v, float* m_scale, float* v_scale, double beta1, double beta2, double eps, double grad_scale,
+                       int64_t t, int groups, const double* lr, const double* weight_decay, int64_t seed, double max_norm, int skip_nonfinite,
+                       int64_t* t_dev, const double* lr_dev, float* norm, void* dyn, double* partial, hipStream_t stream);
 /* the moments that the 8-bit codes of `runs` runs stand for, as floats */
 int ss_adamw8_values(const void* m, const void* v, const float* m_scale, const float* v_scale, float* m_out, float* v_out, int64_t runs,
                      hipStream_t stream);

@@ -68,22 +68,29 @@ __host__ __device__ __forceinline__ unsigned mix32(unsigned x) {       // odd mu
 }
 __host__ __device__ __forceinline__ unsigned step_key(unsigned seed, unsigned t) { return mix32(seed ^ mix32(t)); }
 
-// ------------------------------------------------------------------ global norm: one partial sum (double) per chunk
+// ------------------------------------------------------------------ global norm: one partial sum (double) per workgroup
+// A workgroup walks every gridDim-th chunk with a thread's eight vectors of a chunk in flight at once: with one workgroup a chunk the
+// dependent loads before the first element (plan, address) are a third of its life.  81 M floats: 55 us = 5.8 TB/s alone, 84 - 103 us right
+// behind kernels whose writes still drain.
+#define SS_SQNORM_BLOCKS 2048
 template <typename T>
-__global__ __launch_bounds__(256) void multi_sqnorm_kernel(AdamPtrs ptrs, const AdamChunk* __restrict__ plan, int first_tensor, double* __restrict__ partial) {
-    const AdamChunk c = plan[blockIdx.x];
-    const T* __restrict__ g = (const T*)ptrs.g[c.tensor - first_tensor];
-    const int count = g ? c.count : 0;                         // no gradient: nothing to add
-    g += c.start;
+__global__ __launch_bounds__(256) void multi_sqnorm_kernel(AdamPtrs ptrs, const AdamChunk* __restrict__ plan, int chunks, int first_tensor,
+                                                           double* __restrict__ partial) {
     double s = 0.0;
-    for (int o = threadIdx.x * 4; o < count; o += 4 * 1024) {
-        floatx4 v[4];
+    for (int k = blockIdx.x; k < chunks; k += gridDim.x) {
+        const AdamChunk c = plan[k];
+        const T* __restrict__ g = (const T*)ptrs.g[c.tensor - first_tensor];
+        if (!g) continue;                                      // no gradient: nothing to add
+        g += c.start;
+        for (int o = threadIdx.x * 4; o < c.count; o += 8 * 1024) {
+            floatx4 v[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) { const int k = o + u * 1024, n = count - k; v[u] = n > 0 ? load_n(g + k, n) : floatx4{0.f, 0.f, 0.f, 0.f}; }
+            for (int u = 0; u < 8; ++u) { const int e = o + u * 1024, n = c.count - e; v[u] = n > 0 ? load_n(g + e, n) : floatx4{0.f, 0.f, 0.f, 0.f}; }
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < 8; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { const double d = (double)v[u][e]; s = fma(d, d, s); }
+                for (int e = 0; e < 4; ++e) { const double d = (double)v[u][e]; s = fma(d, d, s); }
+        }
     }
     __shared__ double sh[4];
 #pragma unroll
@@ -95,37 +102,39 @@ __global__ __launch_bounds__(256) void multi_sqnorm_kernel(AdamPtrs ptrs, const 
 
 // One workgroup: joins the partial sums in a fixed order, counts the step, and leaves what the update reads.
 struct AdamSchedule { double lr[SS_ADAMW_GROUPS], wd[SS_ADAMW_GROUPS]; };
-__global__ __launch_bounds__(1024) void adamw_prepare_kernel(const double* __restrict__ partial, int64_t chunks, double max_norm, double grad_scale,
+__global__ __launch_bounds__(1024) void adamw_prepare_kernel(const double* __restrict__ partial, int64_t count, double max_norm, double grad_scale,
         double beta1, double beta2, int64_t t_host, int64_t* __restrict__ t_dev, AdamSchedule sched, const double* __restrict__ lr_dev, int groups,
         unsigned seed, int skip_nonfinite, float* __restrict__ norm_out, AdamDyn* __restrict__ dyn) {
     __shared__ double sh[16];
-    __shared__ double bc1_s;
+    __shared__ double bc1_s, bc2_s;
+    __shared__ int64_t t_s;
+    if (threadIdx.x == 64) {                                                // another wave than the one that ends the sum
+        const int64_t t = t_dev ? *t_dev + 1 : t_host;                      // of a skipped step nothing is used
+        t_s = t; bc1_s = 1.0 - pow(beta1, (double)t); bc2_s = 1.0 - pow(beta2, (double)t);
+    }
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < chunks; i += 1024) s += partial[i];
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < count; i += 1024) s += partial[i];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        s = 0.0;
-        for (int i = 0; i < 16; ++i) s += sh[i];
-        const double norm = sqrt(s) * grad_scale;
-        const bool bad = !(norm < __builtin_huge_val());                    // infinite or NaN
-        const int skip = skip_nonfinite && bad;
-        const int64_t t = t_dev ? *t_dev + (skip ? 0 : 1) : t_host;
-        if (t_dev) *t_dev = t;
-        double clip = 1.0;
-        if (max_norm > 0.0) { clip = max_norm / (norm + 1e-6); clip = clip > 1.0 ? 1.0 : clip; }
-        if (norm_out) *norm_out = (float)norm;
-        const double bc2 = 1.0 - pow(beta2, (double)t);
-        bc1_s = 1.0 - pow(beta1, (double)t);
-        dyn->coef = (float)(clip * grad_scale); dyn->rbc2 = (float)(1.0 / sqrt(bc2)); dyn->key = step_key(seed, (unsigned)t); dyn->skip = skip;
-    }
     __syncthreads();
     if ((int)threadIdx.x < groups) {
         const double lr = lr_dev ? lr_dev[threadIdx.x] : sched.lr[threadIdx.x];
         dyn->step[threadIdx.x] = (float)(lr / bc1_s);
         dyn->decay[threadIdx.x] = (float)(1.0 - lr * sched.wd[threadIdx.x]);
+    }
+    if (threadIdx.x == 0) {
+        s = 0.0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s += sh[i];
+        const double norm = sqrt(s) * grad_scale;
+        const int skip = skip_nonfinite && !(norm < __builtin_huge_val());  // infinite or NaN
+        if (t_dev && !skip) *t_dev = t_s;
+        double clip = 1.0;
+        if (max_norm > 0.0) { clip = max_norm / (norm + 1e-6); clip = clip > 1.0 ? 1.0 : clip; }
+        if (norm_out) *norm_out = (float)norm;
+        dyn->coef = (float)(clip * grad_scale); dyn->rbc2 = (float)(1.0 / sqrt(bc2_s)); dyn->key = step_key(seed, (unsigned)t_s); dyn->skip = skip;
     }
 }
 
@@ -198,21 +207,24 @@ __device__ __forceinline__ float grid_m(float c) { return c * c; }
 __device__ __forceinline__ float grid_v(float c) { const float s = c * c; return s * s; }
 
 // t in units of q -> the code below or above, above with probability (t - below) / (above - below); u16 = 0..65535.
-// The square roots only guess: the code is fixed up against the grid itself, so it does not depend on their rounding.
+// The square roots only guess: raised by 2^-22 (v_sqrt_f32 is good to 1 unit, two in a row to 1.5) the guess is the code below or one too
+// high, and a comparison with the grid itself settles it, so the code does not depend on their rounding.
 template <bool SECOND> __device__ __forceinline__ float encode(float t, float u16) {
 #pragma clang fp contract(off)
     const float top = SECOND ? 254.f : 126.f;
     float c = __builtin_amdgcn_sqrtf(t);
     if (SECOND) c = __builtin_amdgcn_sqrtf(c);
-    c = floorf(c);
+    c = fminf(fmaxf(floorf(c * (1.f + 0x1p-22f)), 0.f), top);
     c = (SECOND ? grid_v(c) : grid_m(c)) > t ? c - 1.f : c;
-    c = (SECOND ? grid_v(c + 1.f) : grid_m(c + 1.f)) <= t ? c + 1.f : c;
-    c = fminf(fmaxf(c, 0.f), top);
-    const float below = SECOND ? grid_v(c) : grid_m(c), above = SECOND ? grid_v(c + 1.f) : grid_m(c + 1.f);
+    const float up = c + 1.f, below = SECOND ? grid_v(c) : grid_m(c), above = SECOND ? grid_v(up) : grid_m(up);
     const float gap = above - below, over = t - below, want = u16 * gap;
-    c = over * 65536.f > want ? c + 1.f : c;
-    if (SECOND) c = (c == 0.f && t > 0.f) ? 1.f : c;
+    c = over * 65536.f > want ? up : c;
+    if (SECOND) c = fmaxf(c, t > 0.f ? 1.f : 0.f);
     return c;
+}
+__device__ __forceinline__ float decode_m(unsigned word, int e) {           // sign(c) c^2
+    const float c = (float)((int)(word << (24 - 8 * e)) >> 24);
+    return c * fabsf(c);
 }
 
 template <typename TP, typename TG>
@@ -240,10 +252,8 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamPtrs2 ptrs, const AdamC
         unsigned mx = 0, vx = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int ci = (int)(mw << (24 - 8 * e)) >> 24;
-            const float cu = (float)((vw >> (8 * e)) & 255u);
-            m[e] = (float)(ci * (ci < 0 ? -ci : ci)) * q1;
-            v[e] = grid_v(cu) * q2;
+            m[e] = decode_m(mw, e) * q1;
+            v[e] = grid_v((float)((vw >> (8 * e)) & 255u)) * q2;
             adam_moments(gv[e] * coef, m[e], v[e], a);
             const unsigned bm = __float_as_uint(m[e]) & 0x7fffffffu, bv = __float_as_uint(v[e]) & 0x7fffffffu;
             mx = mx > bm ? mx : bm; vx = vx > bv ? vx : bv;
@@ -280,8 +290,7 @@ __global__ __launch_bounds__(256) void adamw8_values_kernel(const unsigned* __re
         floatx4 a, b;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int ci = (int)(mw << (24 - 8 * e)) >> 24;
-            a[e] = (float)(ci * (ci < 0 ? -ci : ci)) * q1;
+            a[e] = decode_m(mw, e) * q1;
             b[e] = grid_v((float)((vw >> (8 * e)) & 255u)) * q2;
         }
         *(floatx4*)(m + i * 4) = a; *(floatx4*)(v + i * 4) = b;
@@ -300,20 +309,31 @@ static int check_list(const char* who, int count, const void* const* ptr, const 
     return 0;
 }
 
+static int64_t sqnorm_blocks(int64_t chunks) { return chunks < SS_SQNORM_BLOCKS ? chunks : SS_SQNORM_BLOCKS; }
+
+extern "C" int64_t ss_multi_sqnorm_workspace(int count, const int64_t* first_chunk) {
+    int64_t n = 0;
+    for (int i0 = 0; first_chunk && i0 < count; i0 += SS_ADAMW_PTRS)
+        n += sqnorm_blocks(first_chunk[count - i0 < SS_ADAMW_PTRS ? count : i0 + SS_ADAMW_PTRS] - first_chunk[i0]);
+    return n * (int64_t)sizeof(double);
+}
+
 extern "C" int ss_multi_sqnorm(int dtype, int count, const void* const* grads, const int64_t* first_chunk, const void* plan, double* partial,
                                hipStream_t stream) {
     SS_CHECK(dtype == SS_F32 || dtype == SS_BF16, "ss_multi_sqnorm: unsupported dtype code %d", dtype);
     if (int rc = check_list("ss_multi_sqnorm", count, grads, first_chunk, plan, dtype == SS_F32 ? 4 : 2, true)) return rc;
     for (int i0 = 0; i0 < count; i0 += SS_ADAMW_PTRS) {
         const int n = count - i0 < SS_ADAMW_PTRS ? count - i0 : SS_ADAMW_PTRS;
-        const int64_t c0 = first_chunk[i0], nc = first_chunk[i0 + n] - c0;
+        const int64_t c0 = first_chunk[i0], nc = first_chunk[i0 + n] - c0, blocks = sqnorm_blocks(nc);
         if (nc == 0) continue;
         SS_CHECK(partial, "ss_multi_sqnorm: no room for the partial sums");
         AdamPtrs t;
         memset(&t, 0, sizeof(t));
         for (int i = 0; i < n; ++i) t.g[i] = grads[i0 + i];
-        SS_DISPATCH(dtype, hipLaunchKernelGGL((multi_sqnorm_kernel<T>), dim3((unsigned)nc), dim3(256), 0, stream, t, (const AdamChunk*)plan + c0, i0, partial + c0));
+        SS_DISPATCH(dtype, hipLaunchKernelGGL((multi_sqnorm_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, stream, t, (const AdamChunk*)plan + c0, (int)nc,
+                                              i0, partial));
         SS_LAUNCH_CHECK();
+        partial += blocks;
     }
     return 0;
 }
@@ -327,15 +347,15 @@ static int check_hyper(const char* who, int groups, const double* lr, const doub
     return 0;
 }
 
-extern "C" int ss_adamw_prepare(const double* partial, int64_t chunks, double max_norm, double grad_scale, double beta1, double beta2, int64_t t,
+extern "C" int ss_adamw_prepare(const double* partial, int64_t count, double max_norm, double grad_scale, double beta1, double beta2, int64_t t,
                                 int64_t* t_dev, int groups, const double* lr, const double* weight_decay, const double* lr_dev, int64_t seed,
                                 int skip_nonfinite, float* norm, void* dyn, hipStream_t stream) {
     if (int rc = check_hyper("ss_adamw_prepare", groups, lr, weight_decay, beta1, beta2, grad_scale)) return rc;
-    SS_CHECK(dyn && chunks >= 0 && (chunks == 0 || partial) && (t_dev || t >= 1), "ss_adamw_prepare: bad arguments");
+    SS_CHECK(dyn && count >= 0 && (count == 0 || partial) && (t_dev || t >= 1), "ss_adamw_prepare: bad arguments");
     AdamSchedule s;
     memset(&s, 0, sizeof(s));
     for (int i = 0; i < groups; ++i) { s.lr[i] = lr[i]; s.wd[i] = weight_decay[i]; }
-    hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(1024), 0, stream, partial, chunks, max_norm, grad_scale, beta1, beta2, t, t_dev, s, lr_dev,
+    hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(1024), 0, stream, partial, count, max_norm, grad_scale, beta1, beta2, t, t_dev, s, lr_dev,
                        groups, (unsigned)seed, skip_nonfinite, norm, (AdamDyn*)dyn);
     SS_LAUNCH_CHECK();
     return 0;
@@ -379,6 +399,23 @@ extern "C" int ss_adamw_step(int p_dtype, int g_dtype, int bits, int count, void
         SS_LAUNCH_CHECK();
     }
     return 0;
+}
+
+// norm, preparation and update behind one call: a small model's step is the host's time
+extern "C" int ss_adamw_clip_step(int p_dtype, int g_dtype, int bits, int count, void* const* params, const void* const* grads, const int64_t* first_chunk,
+                                  const void* plan, void* m, void* v, float* m_scale, float* v_scale, double beta1, double beta2, double eps,
+                                  double grad_scale, int64_t t, int groups, const double* lr, const double* weight_decay, int64_t seed, double max_norm,
+                                  int skip_nonfinite, int64_t* t_dev, const double* lr_dev, float* norm, void* dyn, double* partial, hipStream_t stream) {
+    SS_CHECK(dyn, "ss_adamw_clip_step: no room for the step's scalars");
+    int64_t sums = 0;
+    if (partial) {
+        if (int rc = ss_multi_sqnorm(g_dtype, count, grads, first_chunk, plan, partial, stream)) return rc;
+        sums = ss_multi_sqnorm_workspace(count, first_chunk) / (int64_t)sizeof(double);
+    }
+    if (int rc = ss_adamw_prepare(partial, sums, max_norm, grad_scale, beta1, beta2, t, t_dev, groups, lr, weight_decay, lr_dev, seed, skip_nonfinite, norm,
+                                  dyn, stream)) return rc;
+    return ss_adamw_step(p_dtype, g_dtype, bits, count, params, grads, first_chunk, plan, m, v, m_scale, v_scale, beta1, beta2, eps, grad_scale, t, groups, lr,
+                         weight_decay, seed, dyn, stream);
 }
 
 extern "C" int ss_adamw8_values(const void* m, const void* v, const float* m_scale, const float* v_scale, float* m_out, float* v_out, int64_t runs,

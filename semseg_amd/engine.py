@@ -14,7 +14,7 @@ in the reference, laid out for one process per MI355X:
 * ``AdamW``  is the optimizer of the encoders' published recipes (``ss_adamw_step``): flat buffers or a list of tensors, moments in 32 or 8
   bits, gradient clipping by the global norm inside the step.
 """
-import ctypes
+import array
 import math
 import torch
 import torch.distributed as dist
@@ -364,6 +364,8 @@ class AdamW:
         self.exp_avg_sq = torch.zeros(n, dtype=v_type, device=self.device)
         self.exp_avg_scale = torch.zeros(runs, device=self.device) if state_bits == 8 else None
         self.exp_avg_sq_scale = torch.zeros(runs, device=self.device) if state_bits == 8 else None
+        self._partial_bytes = lib().ss_multi_sqnorm_workspace(self.plan.count, self.plan.first_chunk)
+        self._dyn_bytes = lib().ss_adamw_dyn_workspace()
         on_device = self.capturable or self.skip_nonfinite
         self._t = 0
         self._t_dev = torch.zeros(1, dtype=torch.int64, device=self.device) if on_device else None
@@ -392,52 +394,52 @@ class AdamW:
         self._lr_dev.copy_(torch.tensor(self._rates(), dtype=torch.float64))
 
     def _addresses(self):
-        """-> gradient type, HOST arrays of the parameters' and gradients' addresses"""
+        """-> gradient type, HOST arrays of the parameters' and gradients' addresses.  Whole-list passes over bound methods: a loop with the
+        same checks takes twice as long, and a step over 200 small tensors is host time."""
         if self.flat is not None:
             f = self.flat
-            return torch.float32, self.plan.pointers(f.data.data_ptr()), self.plan.pointers(f.grad.data_ptr())
-        gt, pa, ga = None, [], []
-        for p, n in zip(self.params, self.numels):
-            g = p.grad
-            if p.dtype != self.dtype or p.device != self.device or p.numel() != n or not p.is_contiguous():
-                raise RuntimeError('AdamW: a parameter changed its type, device, size or layout')
-            pa.append(p.data_ptr())
-            if g is None:
-                ga.append(None)
-                continue
-            if gt is None:
-                gt = g.dtype
-            if g.dtype != gt or gt not in (torch.float32, torch.bfloat16) or g.device != self.device or g.numel() != n or not g.is_contiguous():
-                raise RuntimeError('AdamW: gradients must be contiguous, of one type (float32 or bfloat16) and on the parameters\' device')
-            ga.append(g.data_ptr())
-        return gt or torch.float32, self.plan.pointers(*pa), self.plan.pointers(*ga)
+            return torch.float32, array.array('Q', (f.data.data_ptr(),)), array.array('Q', (f.grad.data_ptr(),))
+        T, ps = torch.Tensor, self.params
+        if list(map(T.numel, ps)) != self.numels or {p.dtype for p in ps} != {self.dtype} or set(map(T.get_device, ps)) != {self.device.index} \
+                or not all(map(T.is_contiguous, ps)):
+            raise RuntimeError('AdamW: a parameter changed its type, device, size or layout')
+        pa = array.array('Q', map(T.data_ptr, ps))
+        grads = [p.grad for p in ps]
+        there = [g for g in grads if g is not None]
+        types = {g.dtype for g in there}
+        if len(types) > 1 or types - {torch.float32, torch.bfloat16} or not all(map(T.is_contiguous, there)) \
+                or set(map(T.get_device, there)) - {self.device.index} \
+                or list(map(T.numel, there)) != (self.numels if len(there) == len(ps) else [n for n, g in zip(self.numels, grads) if g is not None]):
+            raise RuntimeError('AdamW: gradients must be contiguous, of one type (float32 or bfloat16) and like their parameters')
+        ga = array.array('Q', map(T.data_ptr, there) if len(there) == len(ps) else (0 if g is None else g.data_ptr() for g in grads))
+        return types.pop() if types else torch.float32, pa, ga
 
     def step(self, grad_scale=1.0):
         if self.device.type != 'cuda':
             raise RuntimeError('semseg_amd.AdamW: parameters must live on a HIP device (no CPU fallback)')
-        gt, pa, ga = self._addresses()
-        plan, lb, norm, dyn = self.plan, lib(), None, None
-        k = len(self.groups)
-        lr = (ctypes.c_double * k)(*self._rates())
-        wd = (ctypes.c_double * k)(*[self.wd if w is None else w for _, w in self.groups])
+        gt, p_list, g_list = self._addresses()
+        pa, ga = p_list.buffer_info()[0], g_list.buffer_info()[0]
+        plan, norm, k = self.plan, None, len(self.groups)
+        lr = array.array('d', [self.lr * r for r, _ in self.groups])
+        wd = array.array('d', [self.wd if w is None else w for _, w in self.groups])
         b1, b2 = self.betas
-        with torch.cuda.device(self.device):
-            stream = torch.cuda.current_stream().cuda_stream
+        with ops._DeviceGuard(self.device) as stream:
             measured = self.max_grad_norm is not None or self.skip_nonfinite
             if self._t_dev is None:
                 self._t += 1
+            args = (ops._DT[self.dtype], ops._DT[gt], self.state_bits, plan.count, pa, ga, plan.first_chunk, plan.table.data_ptr(), self.exp_avg.data_ptr(),
+                    self.exp_avg_sq.data_ptr(), ops._p(self.exp_avg_scale), ops._p(self.exp_avg_sq_scale), b1, b2, self.eps, grad_scale, self._t, k,
+                    lr.buffer_info()[0], wd.buffer_info()[0], self.seed)
             if measured or self._t_dev is not None:
-                partial = torch.empty(plan.chunks if measured else 0, dtype=torch.float64, device=self.device)
-                dyn = torch.empty(lb.ss_adamw_dyn_workspace(), dtype=torch.uint8, device=self.device)
+                # scratch from the allocator for each step: nothing that two captured steps or two streams could share
+                work = torch.empty(self._partial_bytes + self._dyn_bytes, dtype=torch.uint8, device=self.device)
                 if measured:
                     norm = torch.empty((), dtype=torch.float32, device=self.device)
-                    check(lb.ss_multi_sqnorm(ops._DT[gt], plan.count, ga, plan.first_chunk, plan.table.data_ptr(), partial.data_ptr(), stream))
-                check(lb.ss_adamw_prepare(partial.data_ptr(), partial.numel(), self.max_grad_norm or 0.0, grad_scale, b1, b2, self._t,
-                                          ops._p(self._t_dev), k, lr, wd, ops._p(self._lr_dev), self.seed, int(self.skip_nonfinite), ops._p(norm),
-                                          dyn.data_ptr(), stream))
-            check(lb.ss_adamw_step(ops._DT[self.dtype], ops._DT[gt], self.state_bits, plan.count, pa, ga, plan.first_chunk, plan.table.data_ptr(),
-                                   self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), ops._p(self.exp_avg_scale), ops._p(self.exp_avg_sq_scale), b1, b2,
-                                   self.eps, grad_scale, self._t, k, lr, wd, self.seed, ops._p(dyn), stream))
+                at = work.data_ptr()
+                check(lib().ss_adamw_clip_step(*args, self.max_grad_norm or 0.0, int(self.skip_nonfinite), ops._p(self._t_dev), ops._p(self._lr_dev),
+                                               ops._p(norm), at + self._partial_bytes, at if measured else None, stream))
+            else:
+                check(lib().ss_adamw_step(*args, None, stream))
         weightprep.bump()                                      # the kernel wrote the parameters through a raw pointer
         return norm
 
@@ -445,11 +447,11 @@ class AdamW:
         """-> both moments as float32, in the state's layout (whole runs of 256 per parameter)"""
         if self.state_bits == 32:
             return self.exp_avg, self.exp_avg_sq
-        with torch.cuda.device(self.device):
+        with ops._DeviceGuard(self.device) as stream:
             m = torch.empty(self.exp_avg.numel(), device=self.device)
             v = torch.empty(self.exp_avg.numel(), device=self.device)
             check(lib().ss_adamw8_values(self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), self.exp_avg_scale.data_ptr(), self.exp_avg_sq_scale.data_ptr(),
-                                         m.data_ptr(), v.data_ptr(), self.plan.runs, torch.cuda.current_stream().cuda_stream))
+                                         m.data_ptr(), v.data_ptr(), self.plan.runs, stream))
         return m, v
 
     # ---- checkpointing in torch.optim's layout, parameters in registration order (FlatParams keeps them reversed); with 8-bit moments the

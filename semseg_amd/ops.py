@@ -1905,4 +1905,3 @@ class TensorPlan:
         first = [0, len(rows)] if offsets is not None else first
         self.first_chunk = (ctypes.c_int64 * len(first))(*first)
         self.table = torch.from_numpy(np.array(rows, dtype=np.int64).reshape(-1, 4)).to(device)
-        self.pointers = ctypes.c_void_p * max(self.count, 1)
