@@ -12,7 +12,7 @@ struct ResnormBwdArgs {
     void *dx, *db, *dgate;                            // dgate: per row
     const float* stats;
     const float *post_w, *post_b, *scale, *keep, *pre_w;
-    float *partial, *gate_partial;                    // [blocks][slots][C] column sums; [units][C] of the per-sample gate
+    float *partial, *gate_partial;                    // [blocks][slots][C] column sums; [units][C] of the per-sample gate, none where a unit is a sample
     int lddh, lddy, ldh, ldb, ldg;
     int sample_rows;                                  // rows that `units_per_sample` units cover: one sample's where the gate is per sample, else all
     FastDiv per_sample;
@@ -22,11 +22,12 @@ struct ResnormBwdArgs {
 };
 
 // Slots of `partial`, in this order, those that exist: pre weight, pre bias, post weight, post bias, scale.
-template <int WAVES> __device__ __forceinline__ void flush_columns(float (&acc)[8], float* __restrict__ dst, int C, Cols k, int lpr, float* sh) {
+template <typename D> __device__ __forceinline__ void put(void* dst, int i, float v, bool as_d) { if (as_d) ((D*)dst)[i] = from_f<D>(v); else ((float*)dst)[i] = v; }
+template <int WAVES, typename D = float> __device__ __forceinline__ void flush_columns(float (&acc)[8], void* dst, bool as_d, int C, Cols k, int lpr, float* sh) {
     k = here(k);
     if constexpr (WAVES > 1) {                                               // a thread owns its columns
 #pragma unroll
-        for (int e = 0; e < 8; ++e) if (e >= k.lo && e < k.hi) dst[k.cb + e] = acc[e];
+        for (int e = 0; e < 8; ++e) if (e >= k.lo && e < k.hi) put<D>(dst, k.cb + e, acc[e], as_d);
     } else {
         const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -37,7 +38,7 @@ template <int WAVES> __device__ __forceinline__ void flush_columns(float (&acc)[
             for (int e = 0; e < 8; ++e) if (e >= k.lo && e < k.hi) sh[(threadIdx.x >> 6) * 512 + k.cb + e] = acc[e];
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < C; i += 256) dst[i] = (sh[i] + sh[512 + i]) + (sh[1024 + i] + sh[1536 + i]);
+        for (int i = threadIdx.x; i < C; i += 256) put<D>(dst, i, (sh[i] + sh[512 + i]) + (sh[1024 + i] + sh[1536 + i]), as_d);
     }
 }
 
@@ -204,19 +205,21 @@ __global__ __launch_bounds__(WAVES > 1 ? WAVES * 64 : 256, WAVES > 4 ? 2 : bwd_w
             work(r1, i + stride);
         }
         if constexpr (GATE == 1) {
-            flush_columns<WAVES>(dgs, a.gate_partial + (int64_t)unit * a.C, a.C, k, lpr, sh);
+            // to the partial sums, or to the gradient itself where the unit is the sample
+            flush_columns<WAVES, TB>(dgs, a.gate_partial ? (void*)(a.gate_partial + (int64_t)unit * a.C) : (void*)((TB*)a.dgate + (int64_t)smp_u * a.C),
+                                     !a.gate_partial, a.C, k, lpr, sh);
 #pragma unroll
             for (int e = 0; e < 8; ++e) dgs[e] = 0.f;
         }
     }
     float* dst = a.partial + (int64_t)blockIdx.x * a.slots * a.C;
-    if (a.pre) { flush_columns<WAVES>(dwp, dst, a.C, k, lpr, sh); dst += a.C; }
-    if (a.pre == 1) { flush_columns<WAVES>(dbp, dst, a.C, k, lpr, sh); dst += a.C; }
+    if (a.pre) { flush_columns<WAVES>(dwp, dst, false, a.C, k, lpr, sh); dst += a.C; }
+    if (a.pre == 1) { flush_columns<WAVES>(dbp, dst, false, a.C, k, lpr, sh); dst += a.C; }
     if constexpr (POST) {
-        flush_columns<WAVES>(dwq, dst, a.C, k, lpr, sh); dst += a.C;
-        if (a.post == 1) { flush_columns<WAVES>(dbq, dst, a.C, k, lpr, sh); dst += a.C; }
+        flush_columns<WAVES>(dwq, dst, false, a.C, k, lpr, sh); dst += a.C;
+        if (a.post == 1) { flush_columns<WAVES>(dbq, dst, false, a.C, k, lpr, sh); dst += a.C; }
     }
-    if (a.scale) flush_columns<WAVES>(dsc, dst, a.C, k, lpr, sh);
+    if (a.scale) flush_columns<WAVES>(dsc, dst, false, a.C, k, lpr, sh);
 }
 
 // Joins the partial sums in a fixed order: workgroup row blockIdx.x < slots is a vector's gradient, the others are samples' gates.
@@ -276,7 +279,7 @@ extern "C" int64_t ss_resnorm_bwd_workspace(int64_t rows, int64_t rows_per_sampl
     int64_t most = 0;                                                        // over the types
     for (int narrow = 0; narrow < 2; ++narrow) {
         const ResnormPlan p = resnorm_plan(rows, rows_per_sample, C, post, pre, gate_mode, has_scale != 0, narrow != 0);
-        const int64_t need = ((int64_t)p.blocks * p.slots + (gate_mode == 1 ? p.units : 0)) * C * 4;
+        const int64_t need = ((int64_t)p.blocks * p.slots + (gate_mode == 1 && p.units_per_sample > 1 ? p.units : 0)) * C * 4;
         if (need > most) most = need;
     }
     return most;
@@ -293,7 +296,7 @@ extern "C" int ss_resnorm_bwd(int x_dtype, int b_dtype, const void* dh, int64_t 
              lddh < SS_RESNORM_MAX_LD && lddy < SS_RESNORM_MAX_LD && ldh < SS_RESNORM_MAX_LD && ldb < SS_RESNORM_MAX_LD && ldg < SS_RESNORM_MAX_LD,
              "ss_resnorm_bwd: bad arguments");
     const ResnormPlan p = resnorm_plan(rows, rows_per_sample, C, post, pre, gate_mode, scale != nullptr, x_dtype == SS_BF16);
-    const int64_t need = ((int64_t)p.blocks * p.slots + (gate_mode == 1 ? p.units : 0)) * C * 4;
+    const int64_t need = ((int64_t)p.blocks * p.slots + (gate_mode == 1 && p.units_per_sample > 1 ? p.units : 0)) * C * 4;
     SS_CHECK((p.slots == 0 || dvec) && (need == 0 || (workspace && ws_bytes >= need)), "ss_resnorm_bwd: workspace too small (%lld of %lld bytes)",
              (long long)ws_bytes, (long long)need);
     ResnormBwdArgs a;
@@ -301,7 +304,7 @@ extern "C" int ss_resnorm_bwd(int x_dtype, int b_dtype, const void* dh, int64_t 
     if (!dh) { dh = h; lddh = ldh; }
     if (!dy) { dy = b; lddy = ldb; h = dh; ldh = lddh; }
     a.dh = dh; a.dy = dy; a.h = h; a.b = b; a.gate = gate; a.dx = dx; a.db = db; a.dgate = dgate; a.stats = stats; a.post_w = post_w; a.post_b = post_b;
-    a.scale = scale; a.keep = keep; a.pre_w = pre_w; a.partial = workspace; a.gate_partial = workspace + (int64_t)p.blocks * p.slots * C;
+    a.scale = scale; a.keep = keep; a.pre_w = pre_w; a.partial = workspace; a.gate_partial = gate_mode == 1 && p.units_per_sample > 1 ? workspace + (int64_t)p.blocks * p.slots * C : nullptr;
     a.lddh = (int)lddh; a.lddy = (int)lddy; a.ldh = (int)ldh; a.ldb = (int)ldb; a.ldg = (int)ldg; a.sample_rows = (int)p.sample_rows;
     a.per_sample = fast_div((unsigned)rows_per_sample); a.units = p.units; a.units_per_sample = p.units_per_sample; a.slots = p.slots;
     a.C = C; a.lpr = p.lpr; a.post = post; a.pre = pre; a.gate_mode = gate_mode; a.act = act; a.alpha = alpha;
@@ -314,7 +317,7 @@ extern "C" int ss_resnorm_bwd(int x_dtype, int b_dtype, const void* dh, int64_t 
         case 4: SS_RN_P(TX, TB, 4); break; default: SS_RN_P(TX, TB, 8); } } while (0)
     if (x_dtype == SS_BF16) SS_RN_W(bf16, bf16); else if (b_dtype == SS_BF16) SS_RN_W(float, bf16); else SS_RN_W(float, float);
     SS_LAUNCH_CHECK();
-    const int64_t join = p.slots + (gate_mode == 1 ? rows / rows_per_sample : 0);
+    const int64_t join = p.slots + (a.gate_partial ? rows / rows_per_sample : 0);
     if (join > 0) {
         const dim3 grid((unsigned)join, (unsigned)cdiv(C, 8));
         if (b_dtype == SS_BF16) hipLaunchKernelGGL(resnorm_join_kernel<bf16>, grid, dim3(256), 0, stream, workspace, p.blocks, p.slots, dvec,

@@ -316,8 +316,9 @@ class AdamW:
     is an 8-bit code with one scale per 256 elements, stored by a draw between two neighbours that depends on (seed, step, element)
     only: 16 instead of 28 bytes per parameter and step.  ``skip_nonfinite``: a step whose gradient norm is infinite or NaN changes nothing
     and is not counted.  ``capturable``: ``step()`` may be captured into a graph; the step count lives on the device, the learning rate
-    is read from there too (``push_lr()`` after moving ``lr`` between replays; betas and decay are captured as they are).  After replays call
-    ``weightprep.bump()``: the parameters were written behind torch's back.
+    is read from there too (``push_lr()`` after moving ``lr`` between replays, an eager step does it by itself; betas and decay are captured
+    as they are).  After replays call ``weightprep.bump()``: the parameters were written behind torch's back.  bfloat16 parameters are rounded
+    to nearest: an update below half a step of a parameter is lost.
 
     ``lr`` and ``betas`` are plain attributes a scheduler may move (``OneCycleLR``)."""
 
@@ -391,7 +392,8 @@ class AdamW:
         """Copies ``lr`` to the device, where captured steps read it."""
         if self._lr_dev is None:
             raise RuntimeError('AdamW.push_lr: only with capturable=True')
-        self._lr_dev.copy_(torch.tensor(self._rates(), dtype=torch.float64))
+        self._pushed = self._rates()
+        self._lr_dev.copy_(torch.tensor(self._pushed, dtype=torch.float64))
 
     def _addresses(self):
         """-> gradient type, HOST arrays of the parameters' and gradients' addresses.  Whole-list passes over bound methods: a loop with the
@@ -417,6 +419,11 @@ class AdamW:
     def step(self, grad_scale=1.0):
         if self.device.type != 'cuda':
             raise RuntimeError('semseg_amd.AdamW: parameters must live on a HIP device (no CPU fallback)')
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing and not self.capturable:
+            raise RuntimeError('AdamW.step: captured into a graph it would repeat one step for ever; build it with capturable=True')
+        if self.capturable and not capturing and self._rates() != self._pushed:
+            self.push_lr()
         gt, p_list, g_list = self._addresses()
         pa, ga = p_list.buffer_info()[0], g_list.buffer_info()[0]
         plan, norm, k = self.plan, None, len(self.groups)

@@ -51,6 +51,8 @@ class _ResnormFn(GradAwareFunction):
 
     @staticmethod
     def backward(ctx, dh, dy):
+        if torch.is_grad_enabled():
+            raise RuntimeError('gated_residual_norm: no gradients of gradients (create_graph=True) are built')
         if dh is None and dy is None:
             return (None,) * 10
         rows, n, C, mode, post, pre, act, alpha, _ = ctx.cfg

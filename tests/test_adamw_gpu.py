@@ -345,3 +345,37 @@ def test_training_run_of_block_norm_and_optimizer_together():
                 # three blocks of two norms and a product each, some 300 roundings in 32 bits deep
                 assert (p.grad.double().cpu() - P[k].grad).abs().max() <= 300 * U * max(float(P[k].grad.abs().max()), float(P[k].grad.norm())) + 1e-9, k
             opt.step()
+
+
+def test_capture_is_refused_without_a_device_count():
+    params, opt, g = build([(64,)], seed=1, max_grad_norm=1.0)
+    give(params, g, torch.float32)
+    opt.step()
+    torch.cuda.synchronize()
+    before = params[0].detach().clone()
+    with pytest.raises(RuntimeError, match='capturable'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.zeros(1, device='cuda')                      # a graph of something, so that capturing itself is in order
+            opt.step()
+    torch.cuda.synchronize()
+    assert torch.equal(params[0], before) and opt.t == 1
+
+
+def test_an_eager_capturable_step_follows_lr():
+    """the rate moved by a scheduler reaches eager steps without push_lr"""
+    a, opt, g = build([(1000,)], seed=2, lr=1e-2, capturable=True)
+    b, opt2, g2 = build([(1000,)], seed=2, lr=1e-2)
+    for k in range(3):
+        opt.lr = opt2.lr = 1e-2 / (k + 1)
+        give(a, g, torch.float32), give(b, g2, torch.float32)
+        opt.step(), opt2.step()
+    assert torch.equal(a[0], b[0])
+
+
+def test_zero_sized_and_single_element_models():
+    params, opt, g = build([(0,), (1,)], seed=3, max_grad_norm=1.0, state_bits=8)
+    give(params, g, torch.float32)
+    assert float(opt.step()) == pytest.approx(abs(float(params[1].grad)), rel=1e-6)
+    params, opt, g = build([(0,)], seed=3, max_grad_norm=1.0)
+    give(params, g, torch.float32)
+    assert float(opt.step()) == 0.0 and opt.t == 1

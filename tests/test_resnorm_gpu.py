@@ -323,3 +323,35 @@ def test_python_refusals_on_the_device():
     wide = torch.zeros(2, 5000, device='cuda')
     with pytest.raises(RuntimeError, match='C=5000'):
         ops.resnorm_fwd(wide, wide)
+
+
+def test_gradients_of_gradients_are_refused():
+    from semseg_amd.resnorm import GatedResidualNorm
+    m = GatedResidualNorm(16).cuda()
+    x = torch.randn(2, 3, 16, device='cuda', requires_grad=True)
+    h, y = m(x, x * 2)
+    with pytest.raises(RuntimeError, match='gradients of gradients'):
+        torch.autograd.grad(y.square().sum(), x, create_graph=True)
+
+
+@pytest.mark.parametrize('C,types', [(40, (H, H)), (512, (F, F)), (700, (F, H)), (4000, (H, H))])
+@pytest.mark.parametrize('samples,n', [(3000, 2), (900, 7), (770, 1), (2, 1500)])
+def test_gates_of_many_and_of_few_samples(C, types, samples, n):
+    """a workgroup that walks whole samples writes their gates' gradients itself; several that share one leave partial sums"""
+    if C >= 700 and samples > 1000:
+        samples //= 4
+    run_and_check(*make(samples * n, C, *types, seed=n, samples=samples, post='layer', pre='rms', gate='sample', act='sigmoid', keep=True))
+
+
+@pytest.mark.parametrize('dtype', [H, F])
+@pytest.mark.parametrize('C', [40, 100, 384, 512, 768, 1000])
+def test_a_row_has_the_same_bits_in_any_company(C, dtype):
+    """few rows are spread over more lanes each than many: same h, y and statistics"""
+    from semseg_amd import ops
+    t, meta, _, _ = make(20000, C, dtype, dtype, seed=C, post='layer', pre='rms', gate='row')
+    d = {k: None if v is None else v.cuda() for k, v in t.items()}
+    h, y, st = ops.resnorm_fwd(**d, **meta)
+    for lo, hi in ((0, 1), (19990, 20000), (7000, 7300)):
+        part = {k: v if v is None or v.dim() == 1 else v[lo:hi] for k, v in d.items()}
+        h1, y1, st1 = ops.resnorm_fwd(**part, **dict(meta, rows_per_sample=hi - lo))
+        assert torch.equal(h1, h[lo:hi]) and torch.equal(y1, y[lo:hi]) and torch.equal(st1, st[lo:hi])
