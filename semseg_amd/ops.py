@@ -1803,12 +1803,17 @@ class _DeviceGuard:
             self.ctx.__exit__(*exc)
 
 
+def _dense(t, shape):
+    """a new dense tensor of `shape`, t's type and device (empty_like costs a third of empty where it does)"""
+    return torch.empty_like(t) if t.is_contiguous() and t.shape == shape else torch.empty(shape, dtype=t.dtype, device=t.device)
+
+
 def _resnorm_launch_fwd(x, ldx, b, ldb, gate, ldg, mode, act, scale, keep, alpha, post, post_w, post_b, pre, pre_w, pre_b, eps, want_stats, rows, n, C, shape):
     """checked arguments -> h, y of `shape`, stats"""
     dev = x.device
     with _DeviceGuard(dev) as stream:
-        h = torch.empty(shape, dtype=x.dtype, device=dev)
-        y = torch.empty(shape, dtype=b.dtype, device=dev) if pre else None
+        h = _dense(x, shape)
+        y = _dense(b, shape) if pre else None
         stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if want_stats else None
         check(lib().ss_resnorm_fwd(_DT[x.dtype], _DT[b.dtype], x.data_ptr(), ldx, b.data_ptr(), ldb, _p(gate), ldg, mode, act, _p(scale), _p(keep), alpha, post,
                                    _p(post_w), _p(post_b), pre, _p(pre_w), _p(pre_b), eps, h.data_ptr(), _p(y), _p(stats), rows, n, C, stream))
@@ -1821,9 +1826,8 @@ def _resnorm_launch_bwd(dh, lddh, dy, lddy, h, ldh, b, ldb, stats, gate, ldg, mo
     dev = h.device
     slots = (pre != 0) + (pre == 1) + (post != 0) + (post == 1) + (scale is not None)
     with _DeviceGuard(dev) as stream:
-        dx = torch.empty(shape, dtype=h.dtype, device=dev)
-        db = torch.empty(shape, dtype=b.dtype, device=dev)
-        dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if mode else None
+        dx, db = _dense(h, shape), _dense(b, shape)
+        dgate = _dense(gate, gate.shape) if mode else None
         # the vectors' gradients and, behind them, the partial sums: from the allocator, not from the shared workspace, since two captured
         # graphs may replay side by side
         need = lib().ss_resnorm_bwd_workspace(rows, n, C, post, pre, mode, int(scale is not None))
@@ -1832,7 +1836,7 @@ def _resnorm_launch_bwd(dh, lddh, dy, lddy, h, ldh, b, ldb, stats, gate, ldg, mo
         check(lib().ss_resnorm_bwd(_DT[h.dtype], _DT[b.dtype], _p(dh), lddh, _p(dy), lddy, h.data_ptr(), ldh, b.data_ptr(), ldb, _p(gate), ldg, mode, act,
                                    _p(scale), _p(keep), alpha, post, _p(post_w), _p(post_b), pre, _p(pre_w), stats.data_ptr(), dx.data_ptr(), db.data_ptr(),
                                    _p(dgate), base, rows, n, C, base + slots * C * 4, need, stream))
-    return dx, db, dgate, buf[:slots * C].view(slots, C) if slots else buf
+    return dx, db, dgate, buf.as_strided((slots, C), (C, 1))
 
 
 def _resnorm_slots(post, pre, scale):
