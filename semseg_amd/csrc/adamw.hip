@@ -72,7 +72,8 @@ __host__ __device__ __forceinline__ unsigned step_key(unsigned seed, unsigned t)
 // A workgroup walks every gridDim-th chunk with a thread's eight vectors of a chunk in flight at once: with one workgroup a chunk the
 // dependent loads before the first element (plan, address) are a third of its life.  81 M floats: 55 us = 5.8 TB/s alone, 84 - 103 us right
 // behind kernels whose writes still drain.
-#define SS_SQNORM_BLOCKS 2048
+#define SS_SQNORM_BLOCKS 1024
+#define SS_ADAMW_JOIN_CHUNKS 4096
 template <typename T>
 __global__ __launch_bounds__(256) void multi_sqnorm_kernel(AdamPtrs ptrs, const AdamChunk* __restrict__ plan, int chunks, int first_tensor,
                                                            double* __restrict__ partial) {
@@ -100,47 +101,69 @@ __global__ __launch_bounds__(256) void multi_sqnorm_kernel(AdamPtrs ptrs, const 
     if (threadIdx.x == 0) partial[blockIdx.x] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
 }
 
+struct AdamArgs {
+    float b1, omb1, b2, omb2, eps;
+    int sums;                                                  // partial sums of the norm, joined by every workgroup (small models)
+    const double* partial;
+    double max_norm, grad_scale;
+    float* norm;
+    AdamDyn dyn;
+};
+
+// Sum of up to a few thousand doubles by a workgroup of 256, in one order wherever it is taken
+__device__ __forceinline__ double join_sums(const double* __restrict__ partial, int64_t count, double* sh) {
+    double s = 0.0;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < count; i += 256) s += partial[i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+    __syncthreads();
+    return (sh[0] + sh[1]) + (sh[2] + sh[3]);
+}
+__device__ __forceinline__ float clip_coef(double norm, double max_norm, double grad_scale) {
+    double clip = 1.0;
+    if (max_norm > 0.0) { clip = max_norm / (norm + 1e-6); clip = clip > 1.0 ? 1.0 : clip; }        // NaN stays NaN
+    return (float)(clip * grad_scale);
+}
+// What the gradients are multiplied by: made by adamw_prepare_kernel, joined here, or given
+__device__ __forceinline__ float step_coef(const AdamArgs& a, const AdamDyn* __restrict__ dyn, bool writes) {
+    if (dyn) return dyn->coef;
+    if (!a.partial) return a.dyn.coef;
+    __shared__ double sh[4];
+    const double norm = sqrt(join_sums(a.partial, a.sums, sh)) * a.grad_scale;
+    if (writes && a.norm && threadIdx.x == 0) *a.norm = (float)norm;
+    return clip_coef(norm, a.max_norm, a.grad_scale);
+}
+
 // One workgroup: joins the partial sums in a fixed order, counts the step, and leaves what the update reads.
 struct AdamSchedule { double lr[SS_ADAMW_GROUPS], wd[SS_ADAMW_GROUPS]; };
-__global__ __launch_bounds__(1024) void adamw_prepare_kernel(const double* __restrict__ partial, int64_t count, double max_norm, double grad_scale,
+__global__ __launch_bounds__(256) void adamw_prepare_kernel(const double* __restrict__ partial, int64_t count, double max_norm, double grad_scale,
         double beta1, double beta2, int64_t t_host, int64_t* __restrict__ t_dev, AdamSchedule sched, const double* __restrict__ lr_dev, int groups,
         unsigned seed, int skip_nonfinite, float* __restrict__ norm_out, AdamDyn* __restrict__ dyn) {
-    __shared__ double sh[16];
+    __shared__ double sh[4];
     __shared__ double bc1_s, bc2_s;
     __shared__ int64_t t_s;
     if (threadIdx.x == 64) {                                                // another wave than the one that ends the sum
         const int64_t t = t_dev ? *t_dev + 1 : t_host;                      // of a skipped step nothing is used
         t_s = t; bc1_s = 1.0 - pow(beta1, (double)t); bc2_s = 1.0 - pow(beta2, (double)t);
     }
-    double s = 0.0;
-#pragma unroll 4
-    for (int64_t i = threadIdx.x; i < count; i += 1024) s += partial[i];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
-    __syncthreads();
+    const double sum = join_sums(partial, count, sh);                       // its barrier also publishes what the other wave made
     if ((int)threadIdx.x < groups) {
         const double lr = lr_dev ? lr_dev[threadIdx.x] : sched.lr[threadIdx.x];
         dyn->step[threadIdx.x] = (float)(lr / bc1_s);
         dyn->decay[threadIdx.x] = (float)(1.0 - lr * sched.wd[threadIdx.x]);
     }
     if (threadIdx.x == 0) {
-        s = 0.0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s += sh[i];
-        const double norm = sqrt(s) * grad_scale;
+        const double norm = sqrt(sum) * grad_scale;
         const int skip = skip_nonfinite && !(norm < __builtin_huge_val());  // infinite or NaN
         if (t_dev && !skip) *t_dev = t_s;
-        double clip = 1.0;
-        if (max_norm > 0.0) { clip = max_norm / (norm + 1e-6); clip = clip > 1.0 ? 1.0 : clip; }
         if (norm_out) *norm_out = (float)norm;
-        dyn->coef = (float)(clip * grad_scale); dyn->rbc2 = (float)(1.0 / sqrt(bc2_s)); dyn->key = step_key(seed, (unsigned)t_s); dyn->skip = skip;
+        dyn->coef = clip_coef(norm, max_norm, grad_scale); dyn->rbc2 = (float)(1.0 / sqrt(bc2_s)); dyn->key = step_key(seed, (unsigned)t_s); dyn->skip = skip;
     }
 }
 
 // ------------------------------------------------------------------ the update
-struct AdamArgs { float b1, omb1, b2, omb2, eps; AdamDyn dyn; };
-
 __device__ __forceinline__ float adam_update(float p, float m, float v, float step, float decay, float rbc2, float eps) {
     const float denom = fmaf(__builtin_amdgcn_sqrtf(v), rbc2, eps);         // v_sqrt_f32 and v_rcp_f32: 1 ulp each of a term far below p
     return p * decay - step * m * __builtin_amdgcn_rcpf(denom);
@@ -161,7 +184,7 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamPtrs2 ptrs, const Adam
         float* __restrict__ v, AdamArgs a, const AdamDyn* __restrict__ dyn) {
     if (dyn && dyn->skip) return;
     const AdamChunk c = plan[blockIdx.x];
-    const float coef = dyn ? dyn->coef : a.dyn.coef, rbc2 = dyn ? dyn->rbc2 : a.dyn.rbc2;
+    const float coef = step_coef(a, dyn, first_tensor == 0 && blockIdx.x == 0), rbc2 = dyn ? dyn->rbc2 : a.dyn.rbc2;
     const float step = dyn ? dyn->step[c.group] : a.dyn.step[c.group], decay = dyn ? dyn->decay[c.group] : a.dyn.decay[c.group];
     const TG* __restrict__ g = (const TG*)ptrs.g[c.tensor - first_tensor];
     if (!g) return;                                            // no gradient: the tensor and its moments stay
@@ -217,7 +240,7 @@ template <bool SECOND> __device__ __forceinline__ float encode(float t, float u1
     c = fminf(fmaxf(floorf(c * (1.f + 0x1p-22f)), 0.f), top);
     c = (SECOND ? grid_v(c) : grid_m(c)) > t ? c - 1.f : c;
     const float up = c + 1.f, below = SECOND ? grid_v(c) : grid_m(c), above = SECOND ? grid_v(up) : grid_m(up);
-    const float gap = above - below, over = t - below, want = u16 * gap;
+    const float gap = SECOND ? above - below : up + c, over = t - below, want = u16 * gap;
     c = over * 65536.f > want ? up : c;
     if (SECOND) c = fmaxf(c, t > 0.f ? 1.f : 0.f);
     return c;
@@ -232,7 +255,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamPtrs2 ptrs, const AdamC
         unsigned* __restrict__ vc, float* __restrict__ qm, float* __restrict__ qv, AdamArgs a, const AdamDyn* __restrict__ dyn) {
     if (dyn && dyn->skip) return;
     const AdamChunk c = plan[blockIdx.x];
-    const float coef = dyn ? dyn->coef : a.dyn.coef, rbc2 = dyn ? dyn->rbc2 : a.dyn.rbc2;
+    const float coef = step_coef(a, dyn, first_tensor == 0 && blockIdx.x == 0), rbc2 = dyn ? dyn->rbc2 : a.dyn.rbc2;
     const float step = dyn ? dyn->step[c.group] : a.dyn.step[c.group], decay = dyn ? dyn->decay[c.group] : a.dyn.decay[c.group];
     const unsigned key = dyn ? dyn->key : a.dyn.key;
     const TG* __restrict__ g = (const TG*)ptrs.g[c.tensor - first_tensor];
@@ -271,7 +294,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamPtrs2 ptrs, const AdamC
             const unsigned h = mix32(rk + (unsigned)(lane * 4 + e) * 0x9E3779B9u);
             const float cm = encode<false>(fabsf(m[e]) * i1, (float)(h & 0xffffu));
             const float cv = encode<true>(v[e] * i2, (float)(h >> 16));
-            const int ci = (int)(m[e] < 0.f ? -cm : cm);
+            const int ci = (int)copysignf(cm, m[e]);
             mo |= ((unsigned)ci & 255u) << (8 * e);
             vo |= (unsigned)cv << (8 * e);
         }
@@ -355,16 +378,17 @@ extern "C" int ss_adamw_prepare(const double* partial, int64_t count, double max
     AdamSchedule s;
     memset(&s, 0, sizeof(s));
     for (int i = 0; i < groups; ++i) { s.lr[i] = lr[i]; s.wd[i] = weight_decay[i]; }
-    hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(1024), 0, stream, partial, count, max_norm, grad_scale, beta1, beta2, t, t_dev, s, lr_dev,
+    hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(256), 0, stream, partial, count, max_norm, grad_scale, beta1, beta2, t, t_dev, s, lr_dev,
                        groups, (unsigned)seed, skip_nonfinite, norm, (AdamDyn*)dyn);
     SS_LAUNCH_CHECK();
     return 0;
 }
 
-extern "C" int ss_adamw_step(int p_dtype, int g_dtype, int bits, int count, void* const* params, const void* const* grads, const int64_t* first_chunk,
+struct AdamNorm { const double* partial; int sums; double max_norm; float* norm; };
+static int adamw_step(int p_dtype, int g_dtype, int bits, int count, void* const* params, const void* const* grads, const int64_t* first_chunk,
                              const void* plan, void* m, void* v, float* m_scale, float* v_scale, double beta1, double beta2, double eps,
                              double grad_scale, int64_t t, int groups, const double* lr, const double* weight_decay, int64_t seed, const void* dyn,
-                             hipStream_t stream) {
+                      const AdamNorm& joined, hipStream_t stream) {
     SS_CHECK((p_dtype == SS_F32 || p_dtype == SS_BF16) && (g_dtype == SS_F32 || g_dtype == SS_BF16), "ss_adamw_step: unsupported dtype codes %d / %d", p_dtype, g_dtype);
     SS_CHECK(bits == 32 || bits == 8, "ss_adamw_step: moments of 32 or 8 bits, got %d", bits);
     if (int rc = check_hyper("ss_adamw_step", groups, lr, weight_decay, beta1, beta2, grad_scale)) return rc;
@@ -376,6 +400,7 @@ extern "C" int ss_adamw_step(int p_dtype, int g_dtype, int bits, int count, void
     AdamArgs a;
     memset(&a, 0, sizeof(a));
     a.b1 = (float)beta1; a.omb1 = (float)(1.0 - beta1); a.b2 = (float)beta2; a.omb2 = (float)(1.0 - beta2); a.eps = (float)eps;   // each rounded once
+    a.partial = joined.partial; a.sums = joined.sums; a.max_norm = joined.max_norm; a.grad_scale = grad_scale; a.norm = joined.norm;
     if (!dyn) {
         const double bc1 = 1.0 - pow(beta1, (double)t), bc2 = 1.0 - pow(beta2, (double)t);
         a.dyn.coef = (float)grad_scale; a.dyn.rbc2 = (float)(1.0 / sqrt(bc2)); a.dyn.key = step_key((unsigned)seed, (unsigned)t);
@@ -401,6 +426,14 @@ extern "C" int ss_adamw_step(int p_dtype, int g_dtype, int bits, int count, void
     return 0;
 }
 
+extern "C" int ss_adamw_step(int p_dtype, int g_dtype, int bits, int count, void* const* params, const void* const* grads, const int64_t* first_chunk,
+                             const void* plan, void* m, void* v, float* m_scale, float* v_scale, double beta1, double beta2, double eps,
+                             double grad_scale, int64_t t, int groups, const double* lr, const double* weight_decay, int64_t seed, const void* dyn,
+                             hipStream_t stream) {
+    return adamw_step(p_dtype, g_dtype, bits, count, params, grads, first_chunk, plan, m, v, m_scale, v_scale, beta1, beta2, eps, grad_scale, t, groups, lr,
+                      weight_decay, seed, dyn, AdamNorm{nullptr, 0, 0.0, nullptr}, stream);
+}
+
 // norm, preparation and update behind one call: a small model's step is the host's time
 extern "C" int ss_adamw_clip_step(int p_dtype, int g_dtype, int bits, int count, void* const* params, const void* const* grads, const int64_t* first_chunk,
                                   const void* plan, void* m, void* v, float* m_scale, float* v_scale, double beta1, double beta2, double eps,
@@ -411,6 +444,12 @@ extern "C" int ss_adamw_clip_step(int p_dtype, int g_dtype, int bits, int count,
     if (partial) {
         if (int rc = ss_multi_sqnorm(g_dtype, count, grads, first_chunk, plan, partial, stream)) return rc;
         sums = ss_multi_sqnorm_workspace(count, first_chunk) / (int64_t)sizeof(double);
+    }
+    // few chunks: every workgroup joins the partial sums itself, which saves a launch of 4 us; many would read them too often
+    if (partial && !t_dev && !lr_dev && !skip_nonfinite && count > 0 && first_chunk[count] > 0 && first_chunk[count] <= SS_ADAMW_JOIN_CHUNKS) {
+        SS_CHECK(max_norm > 0.0 || norm, "ss_adamw_clip_step: a norm that nobody asked for");
+        return adamw_step(p_dtype, g_dtype, bits, count, params, grads, first_chunk, plan, m, v, m_scale, v_scale, beta1, beta2, eps, grad_scale, t, groups,
+                          lr, weight_decay, seed, nullptr, AdamNorm{partial, (int)sums, max_norm, norm}, stream);
     }
     if (int rc = ss_adamw_prepare(partial, sums, max_norm, grad_scale, beta1, beta2, t, t_dev, groups, lr, weight_decay, lr_dev, seed, skip_nonfinite, norm,
                                   dyn, stream)) return rc;

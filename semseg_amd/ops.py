@@ -1888,10 +1888,9 @@ class TensorPlan:
         import numpy as np
         numels = [int(n) for n in numels]
         groups = [0] * len(numels) if groups is None else list(groups)
-        total = sum(numels)
-        # about eight workgroups a CU where there is that much; 1024 elements (four a thread) at least
+        # one round of the eight workgroups a CU holds if chunks of up to 8192 elements allow it; 1024 elements, four a thread, at least
         chunk = 1024
-        while chunk < 8192 and total > chunk * 2048:
+        while chunk < 8192 and sum(-(-n // chunk) for n in numels) > 2048:
             chunk *= 2
         rows, first, self.first_run, run = [], [0], [], 0
         for i, n in enumerate(numels):
