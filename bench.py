@@ -50,6 +50,8 @@ def parse():
     ap.add_argument('--shapes', action='store_true', help='print per-shape GEMM / attention timings to stderr')
     ap.add_argument('--train', action='store_true', help='topformer: the training step of train.py:45-52 (TopFormer-B, fwd + OHEM-CE + confusion '
                     'matrix + bwd + grad all-reduce + AdaBound; default 1024x1024, batch 16) instead of configs[3] inference')
+    ap.add_argument('--optimizer', default='adabound', choices=['adabound', 'adamw', 'adamw8'], help='training workloads: AdaBound as train.py:53-58 '
+                    '(the headline), or AdamW with the gradient clipped to norm 1, moments in 32 or in 8 bits, no decay of vectors')
     ap.add_argument('--force-comm', action='store_true', help='N = 1: create the RCCL process group (world size 1) and run the bucketed '
                     'all-reduce path (side stream, hooks, collectives) anyway, so the real backend is exercised on one GPU')
     return ap.parse_args()
@@ -440,7 +442,7 @@ def main():
     from semseg_amd.metrics import SegmentationMetrics
     from semseg_amd.detinit import det_fill_
     from semseg_amd.runtime import set_compute_dtype
-    from semseg_amd.engine import FlatParams, GradReducer, AdaBound, broadcast_module_state
+    from semseg_amd.engine import FlatParams, GradReducer, AdaBound, AdamW, broadcast_module_state
     from semseg_amd import _lib
 
     T = torch.bfloat16 if a.dtype == 'bf16' else torch.float32
@@ -461,7 +463,11 @@ def main():
     broadcast_module_state(net)
     flat = FlatParams(net)
     reducer = GradReducer(flat, force_comm=a.force_comm)
-    opt = AdaBound(flat, lr=1e-3, final_lr=0.1)
+    if a.optimizer == 'adabound':
+        opt = AdaBound(flat, lr=1e-3, final_lr=0.1)
+    else:
+        opt = AdamW(flat, lr=6e-5, weight_decay=0.01, max_grad_norm=1.0, state_bits=8 if a.optimizer == 'adamw8' else 32,
+                    per_param=lambda p: {'weight_decay': 0.0} if p.dim() <= 1 else {})
     if a.workload == 'dnet':
         crit = DiceLoss(0.5, False, 6)
     elif a.loss == 'ce_dice':
@@ -531,16 +537,17 @@ def main():
             dist.destroy_process_group()
         return
     ms = 1e3 * dt / a.steps
+    optim = {'adabound': 'AdaBound', 'adamw': 'AdamW', 'adamw8': 'AdamW (8-bit moments)'}[a.optimizer]
     what = {'dnet': 'DNet ConvNeXt-T', 'topformer': f'TopFormer-B + {a.head} head'}.get(a.workload, f'MiT-{a.variant}+Lawin')
     res = {'metric': f'train images/sec @{a.size}x{a.size} ({what})', 'value': a.batch * world * a.steps / dt, 'unit': 'images/s',
            'n_gpus': world, 'steps': a.steps, 'warmup': a.warmup, 'ms_per_step': ms, 'higher_is_better': True, 'scaling': 'weak',
            'vs_baseline': None, 'dtype': a.dtype, 'data': 'synthetic',
            'config': {'workload': (f'configs[2] per-GPU step: DNet(ConvNeXt-T + Decoder(embed 256), 6 cls) training step (fwd + Dice + confusion '
-                                   f'matrix + bwd + grad all-reduce + AdaBound), {a.size}x{a.size}') if a.workload == 'dnet' else
+                                   f'matrix + bwd + grad all-reduce + {optim}), {a.size}x{a.size}') if a.workload == 'dnet' else
                                   (f'train.py:45-52 model: TopFormer-B + {a.head} head (6 cls) training step (fwd + OHEM-CE + confusion matrix + bwd + '
-                                   f'grad all-reduce + AdaBound), {a.size}x{a.size}') if a.workload == 'topformer' else
+                                   f'grad all-reduce + {optim}), {a.size}x{a.size}') if a.workload == 'topformer' else
                                   f'configs[1]: SegFormer MiT-{a.variant} + LawinHead({a.embed}, 6 cls) training step '
-                                  f'(fwd + {"OHEM-CE + Dice" if a.loss == "ce_dice" else "OHEM-CE"} + confusion matrix + bwd + grad all-reduce + AdaBound), {a.size}x{a.size}',
+                                  f'(fwd + {"OHEM-CE + Dice" if a.loss == "ce_dice" else "OHEM-CE"} + confusion matrix + bwd + grad all-reduce + {optim}), {a.size}x{a.size}',
                       'per_gpu_batch': a.batch, 'global_batch': a.batch * world, 'parallelism': f'dp{world}',
                       'weights': 'deterministic random init'},
            'loss': float(loss.detach()), 'mIoU': float(cm['mIoU']), 'peak_mem_gib': torch.cuda.max_memory_allocated() / 2 ** 30}
@@ -549,7 +556,7 @@ def main():
     if comm is not None:
         res['communicator'] = comm
     if table is not None:                                        # the rate with the optimizer step excluded, beside `value`
-        opt_ms = sum(t['ms'] for name, t in table.items() if 'adabound' in name)
+        opt_ms = sum(t['ms'] for name, t in table.items() if 'adabound' in name or 'adamw' in name)
         res['optimizer_ms_per_step'] = opt_ms
         res['value_without_optimizer'] = a.batch * world / ((ms - opt_ms) * 1e-3)
     if table is not None and a.table:
