@@ -21,10 +21,11 @@ template <> struct Chunk<float> {
     __device__ __forceinline__ void set(int e, float f) { if (e < 4) a[e & 3] = f; else b[e & 3] = f; }
     __device__ __forceinline__ void store(float* p) const { ((Fl8u*)p)->a = a; ((Fl8u*)p)->b = b; }
 };
-// The eight channels of a lane: [cb, cb + 8), of which e in [lo, hi) are its own.  At the end of a row whose width is no multiple of eight
-// the last chunk is moved back to end with the row, and a lane past the row's end reads that chunk too and owns nothing: every load is a
-// whole chunk inside the row, without a branch.  (A load under a branch may not have been issued, so a wait for an older one has to
-// wait for everything, and the next row's loads are not in flight any more: ConvNeXt stage 3 backward 101 us against 75.)
+// The eight channels of a lane: [cb, cb + 8), of which e in [lo, hi) count as its own.  At the end of a row whose width is no multiple of
+// eight the last chunk is moved back to end with the row, and a lane past the row's end reads that chunk too and owns nothing: every load
+// is a whole chunk inside the row, without a branch.  (A load under a branch may not have been issued, so a wait for an older one has to
+// wait for everything, and the next row's loads are not in flight any more: ConvNeXt stage 3 backward 101 us against 75.)  What two lanes
+// hold of the same channel is the same to the last bit, so the moved chunk is stored whole as well; only sums count a channel once.
 struct Cols { int cb, lo, hi; };
 __device__ __forceinline__ Cols cols_of(int c, int C) {
     const int n = C - c;
@@ -44,11 +45,10 @@ template <typename T> __device__ __forceinline__ void load_chunk(Chunk<T>& t, co
         for (int e = 0; e < 8; ++e) t.set(e, to_f(p[e < C ? e : C - 1]));
     }
 }
-template <typename T> __device__ __forceinline__ void store_chunk(const Chunk<T>& t, T* p, const Cols& k) {
-    if (k.lo == 0 && k.hi == 8) { t.store(p); return; }
-    const Cols own = here(k);
+template <typename T> __device__ __forceinline__ void store_chunk(const Chunk<T>& t, T* p, int C) {
+    if (C >= 8) { t.store(p); return; }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) if (e >= own.lo && e < own.hi) p[e] = from_f<T>(t.get(e));
+    for (int e = 0; e < 7; ++e) if (e < C) p[e] = from_f<T>(t.get(e));
 }
 
 // Address of a lane's element: a row that the whole wave agrees on (64 bits, scalar registers) and the lane's offset from it (32 bits): one
@@ -107,27 +107,19 @@ template <int WAVES> __device__ __forceinline__ void row_stats(double s, double 
 __device__ __forceinline__ float sigmoid_f(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 
 // ---------------------------------------------------------------- the vectors (weights, biases, scale) in LDS
-// One row of `chunks` chunks per vector, the two halves of a chunk apart: lanes read 16 bytes each, 16 bytes apart.  Where a chunk's channel
-// is not the lane's own the vectors are ZERO.
-__device__ __forceinline__ float vec_value(const float* p, float otherwise, int C, int i) {
-    const Cols k = cols_of(i & ~7, C);
-    const int e = i & 7;
-    return e < k.lo || e >= k.hi ? 0.f : p ? p[k.cb + e] : otherwise;
-}
+// One row of `chunks` chunks per vector, the two halves of a chunk apart: lanes read 16 bytes each, 16 bytes apart.
 __device__ __forceinline__ void stage_vec(float* sh, const float* p, float otherwise, int C, int chunks, int threads) {
-    for (int i = threadIdx.x; i < chunks * 8; i += threads) sh[((i >> 2) & 1) * chunks * 4 + (i >> 3) * 4 + (i & 3)] = vec_value(p, otherwise, C, i);
-}
-// the same for a thread that owns its columns
-__device__ __forceinline__ void load_vec(float (&v)[8], const float* p, float otherwise, const Cols& k) {
-    if (p) {
-        Chunk<float> t;
-        t.load(p + k.cb);                                                    // C > 8 here
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < k.lo ? 0.f : t.get(e);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < k.lo ? 0.f : otherwise;
+    for (int i = threadIdx.x; i < chunks * 8; i += threads) {
+        const int c = cols_of(i & ~7, C).cb + (i & 7);
+        sh[((i >> 2) & 1) * chunks * 4 + (i >> 3) * 4 + (i & 3)] = c >= C ? 0.f : p ? p[c] : otherwise;
     }
+}
+// the same for a thread that owns its columns (C > 8)
+__device__ __forceinline__ void load_vec(float (&v)[8], const float* p, float otherwise, const Cols& k) {
+    Chunk<float> t;
+    if (p) t.load(p + k.cb);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = p ? t.get(e) : otherwise;
 }
 __device__ __forceinline__ void vec_chunk(float (&v)[8], const float* sh, int chunk, int chunks) {
     const floatx4 a = *(const floatx4*)(sh + chunk * 4), b = *(const floatx4*)(sh + chunks * 4 + chunk * 4);

@@ -28,18 +28,12 @@ struct ResnormArgs {
     int ldx, ldb, ldg, rows;
     FastDiv per_sample;                               // rows of one sample
     double inv_c;
-    int ragged;                                       // some lane owns less than eight channels
+    int ragged;                                       // 1: some lane owns nothing; 2: one owns less than eight channels
     int C, lpr, post, pre, gate_mode, act;            // norms: 0 none, 1 LayerNorm, 2 RMSNorm; gate: 0 none, 1 per sample, 2 per row
     float alpha;
     double eps;
 };
 
-// what is not the lane's own is no part of its row's sums
-__device__ __forceinline__ void keep_own(float (&v)[8], Cols k) {
-    k = here(k);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < k.lo || e >= k.hi ? 0.f : v[e];
-}
 // One lane's part of a row: NCH chunks of 8 channels
 template <typename TX, typename TB, int NCH, bool GATE> struct FwdRow { Chunk<TX> x[NCH]; Chunk<TB> b[NCH], g[GATE ? NCH : 1]; float keep; };
 
@@ -93,6 +87,22 @@ __global__ __launch_bounds__(WAVES > 1 ? WAVES * 64 : 256) void resnorm_fwd_kern
             for (int e = 0; e < 8; ++e) v[e] = own[which][e];
         } else vec_chunk(v, vec + which * vlen, lig + j * lpr, chunks);
     };
+    auto sums = [&](const float (&f)[NCH][8], double& s, double& q) {        // a channel counts once
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            double cs = 0.0, cq = 0.0;
+            if (a.ragged == 2) {
+                const Cols k = here(cols_of((lig + j * lpr) * 8, a.C));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { const float v = e < k.lo || e >= k.hi ? 0.f : f[j][e]; const double d = (double)v; cs += d; cq = __builtin_fma(d, d, cq); }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { const double d = (double)f[j][e]; cs += d; cq = __builtin_fma(d, d, cq); }
+                if (a.ragged && (lig + j * lpr) * 8 >= a.C) { cs = 0.0; cq = 0.0; }
+            }
+            s += cs; q += cq;
+        }
+    };
     auto work = [&](const FwdRow<TX, TB, NCH, GATE != 0>& t, int i) {
 #pragma clang fp contract(off)
         const int row = first + i;
@@ -104,15 +114,8 @@ __global__ __launch_bounds__(WAVES > 1 ? WAVES * 64 : 256) void resnorm_fwd_kern
                 for (int e = 0; e < 8; ++e) f[j][e] = t.b[j].get(e);
             float mu = 0.f, r = 0.f, mh = 0.f, rh = 0.f;
             if constexpr (POST) {
-                if (a.ragged) {
-#pragma unroll
-                    for (int j = 0; j < NCH; ++j) keep_own(f[j], cols_of((lig + j * lpr) * 8, a.C));
-                }
                 double s = 0.0, q = 0.0;
-#pragma unroll
-                for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) { const double d = (double)f[j][e]; s += d; q = __builtin_fma(d, d, q); }
+                sums(f, s, q);
                 row_stats<WAVES>(s, q, a.post, a.inv_c, a.eps, lanes, sh, turn, mu, r);
 #pragma unroll
                 for (int j = 0; j < NCH; ++j) {
@@ -158,20 +161,13 @@ __global__ __launch_bounds__(WAVES > 1 ? WAVES * 64 : 256) void resnorm_fwd_kern
                 Chunk<TX> hv;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) hv.set(e, t.x[j].get(e) * a.alpha + f[j][e]);
-                if (ok && k.lo < k.hi) store_chunk(hv, at((TX*)a.h, row, a.C, (unsigned)(lr * a.C + k.cb)), k);
+                if (ok && k.lo < k.hi) store_chunk(hv, at((TX*)a.h, row, a.C, (unsigned)(lr * a.C + k.cb)), a.C);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[j][e] = hv.get(e);
             }
             if (a.pre) {
-                if (a.ragged) {
-#pragma unroll
-                    for (int j = 0; j < NCH; ++j) keep_own(f[j], cols_of((lig + j * lpr) * 8, a.C));
-                }
                 double s = 0.0, q = 0.0;
-#pragma unroll
-                for (int j = 0; j < NCH; ++j)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) { const double d = (double)f[j][e]; s += d; q = __builtin_fma(d, d, q); }
+                sums(f, s, q);
                 row_stats<WAVES>(s, q, a.pre, a.inv_c, a.eps, lanes, sh, turn, mh, rh);
 #pragma unroll
                 for (int j = 0; j < NCH; ++j) {
@@ -181,7 +177,7 @@ __global__ __launch_bounds__(WAVES > 1 ? WAVES * 64 : 256) void resnorm_fwd_kern
                     Chunk<TB> yv;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) yv.set(e, (f[j][e] - mh) * rh * w[e] + v[e]);
-                    if (ok && k.lo < k.hi) store_chunk(yv, at((TB*)a.y, row, a.C, (unsigned)(lr * a.C + k.cb)), k);
+                    if (ok && k.lo < k.hi) store_chunk(yv, at((TB*)a.y, row, a.C, (unsigned)(lr * a.C + k.cb)), a.C);
                 }
             }
         if (a.stats && lig == 0 && ok) *at((floatx4*)a.stats, row, 1, (unsigned)lr) = floatx4{mu, r, mh, rh};
@@ -224,14 +220,23 @@ extern "C" int ss_resnorm_fwd(int x_dtype, int b_dtype, const void* x, int64_t l
     a.C = C; a.post = post; a.pre = pre; a.gate_mode = gate_mode; a.act = act; a.alpha = alpha; a.eps = eps; a.inv_c = 1.0 / (double)C;
     const int chunks = (int)cdiv(C, 8);
     int waves = 1, nch = 1;
-    // lanes of a row: eight or sixteen with up to four chunks each (row sums in few steps, no idle lanes at the usual widths) where there are
-    // rows for every SIMD, else a whole wave: 1 row of 512 bf16 6.4 -> 5.0 us, 5223 of 97 f32 9.6 -> 8.2 us
-    const int wide = chunks <= 16 ? 16 : chunks <= 32 ? 32 : 64;
-    if (chunks > 8 && chunks <= 128 && rows * (chunks <= 32 ? 8 : chunks <= 64 ? 16 : 32) < 64 * 1024) { a.lpr = wide; nch = (int)cdiv(chunks, wide); }
-    else if (chunks <= 8) { a.lpr = 1; while (a.lpr < chunks) a.lpr <<= 1; }
-    else if (chunks <= 128) { a.lpr = chunks <= 32 ? 8 : chunks <= 64 ? 16 : 32; nch = (int)cdiv(chunks, a.lpr); }
+    // Lanes of a row, measured at 24 M elements:
+    // - a stream in 32 bits is bound by its bytes: one chunk a lane, whole lines in a load (C = 96: 85 us, 96 in four lanes, 100 in eight;
+    //   320: 80 in 64 lanes, 103 in sixteen), above 512 channels 32 lanes (768: 96, 106 in 64);
+    // - a bf16 stream with norms and gates is bound by vector instructions: up to four chunks a lane so that the fewest lanes are idle, of those
+    //   the most lanes (C = 96 in 4 x 3: 44 us, 53 in 16; 384 in 16 x 3: 43, 57 in 64; 128 in 16: 41, 43 in 8 x 2);
+    // - with rows too few for a wave on every SIMD, as many lanes as there are chunks (1 row of 512: 6.4 -> 5.0 us).
+    const bool wide = x_dtype == SS_F32 || rows * chunks < 64 * 1024;
+    if (chunks <= 64 && wide) { a.lpr = 1; while (a.lpr < chunks) a.lpr <<= 1; }
+    else if (chunks <= 128) {
+        int slots = 1 << 30;
+        for (int l = x_dtype == SS_F32 && rows * chunks >= 64 * 1024 ? 32 : 64; l >= 1; l >>= 1) {
+            const int n = (int)cdiv(chunks, l);
+            if (n <= 4 && l * n < slots) { slots = l * n; a.lpr = l; nch = n; }
+        }
+    }
     else { waves = chunks <= 256 ? 4 : 8; a.lpr = waves * 64; }
-    a.ragged = C != a.lpr * nch * 8;
+    a.ragged = C % 8 ? 2 : C != a.lpr * nch * 8;
     const int64_t want = waves > 1 ? rows : cdiv(rows, 4 * (64 / a.lpr)), most = waves > 1 ? 4096 / waves : 1024;
     const unsigned grid = (unsigned)(want < most ? want : most);
     const size_t shm = waves > 1 ? 0 : (size_t)5 * a.lpr * nch * 8 * sizeof(float);

@@ -6,6 +6,8 @@
 // launch in a fixed order; nothing is atomic.
 #include "resnorm.h"
 
+struct __attribute__((packed, aligned(4))) Fl4u { floatx4 v; };
+
 struct ResnormBwdArgs {
     const void *dh, *dy, *h, *b, *gate;               // one that is not given points at another of its type: it is loaded for nothing, from the cache
     int has_dh, has_dy;
@@ -16,7 +18,7 @@ struct ResnormBwdArgs {
     int lddh, lddy, ldh, ldb, ldg;
     int sample_rows;                                  // rows that `units_per_sample` units cover: one sample's where the gate is per sample, else all
     FastDiv per_sample;
-    int units, units_per_sample, slots;
+    int units, units_per_sample, slots, ragged;       // ragged 1: some lane owns nothing; 2: one owns less than eight channels
     int C, lpr, post, pre, gate_mode, act;
     float alpha;
 };
@@ -65,6 +67,17 @@ __global__ __launch_bounds__(WAVES > 1 ? WAVES * 64 : 256, WAVES > 4 ? 2 : bwd_w
     stage_vec(vec + 2 * vlen, a.scale, 1.f, a.C, lpr, THREADS);
     if (a.pre) stage_vec(vec + 3 * vlen, a.pre_w, 1.f, a.C, lpr, THREADS);
     __syncthreads();
+    auto sums = [&](const float (&g)[8], const float (&hat)[8], float& s1, float& s2) {      // a channel counts once
+        if (a.ragged == 2) {
+            const Cols own = here(k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { const float v = e < own.lo || e >= own.hi ? 0.f : g[e]; s1 += v; s2 = fmaf(v, hat[e], s2); }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { s1 += g[e]; s2 = fmaf(g[e], hat[e], s2); }
+            if (a.ragged && lig * 8 >= a.C) { s1 = 0.f; s2 = 0.f; }
+        }
+    };
     float dwp[8] = {}, dbp[8] = {}, dwq[8] = {}, dbq[8] = {}, dsc[8] = {}, dgs[8] = {};
     for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
         // a unit: every units_per_sample-th step of a sample's rows, so that the workgroups at work read one stretch of memory together
@@ -112,8 +125,8 @@ __global__ __launch_bounds__(WAVES > 1 ? WAVES * 64 : 256, WAVES > 4 ? 2 : bwd_w
                         hat[e] = (t.h.get(e) - mh) * rh;
                         dwp[e] = fmaf(gy, hat[e], dwp[e]); dbp[e] += gy;
                         g[e] = gy * v[e];
-                        s1 += g[e]; s2 = fmaf(g[e], hat[e], s2);
                     }
+                    sums(g, hat, s1, s2);
                     row_sum2<WAVES>(s1, s2, lanes, sh, turn);
                     s1 = a.pre == 1 ? s1 * invC : 0.f; s2 *= invC;
 #pragma unroll
@@ -123,7 +136,7 @@ __global__ __launch_bounds__(WAVES > 1 ? WAVES * 64 : 256, WAVES > 4 ? 2 : bwd_w
                     Chunk<TX> o;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) o.set(e, d[e] * a.alpha);
-                    store_chunk(o, at((TX*)a.dx, row, a.C, dense), k);
+                    store_chunk(o, at((TX*)a.dx, row, a.C, dense), a.C);
                 }
                 // dn, the scale's and the gate's gradients; n = hat w + bias
                 float act[8], nn[8];
@@ -166,7 +179,7 @@ __global__ __launch_bounds__(WAVES > 1 ? WAVES * 64 : 256, WAVES > 4 ? 2 : bwd_w
                         Chunk<TB> o;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) o.set(e, nn[e]);
-                        store_chunk(o, at((TB*)a.dgate, row, a.C, dense), k);
+                        store_chunk(o, at((TB*)a.dgate, row, a.C, dense), a.C);
                     }
                 } else {
 #pragma unroll
@@ -179,8 +192,8 @@ __global__ __launch_bounds__(WAVES > 1 ? WAVES * 64 : 256, WAVES > 4 ? 2 : bwd_w
                     for (int e = 0; e < 8; ++e) {
                         dwq[e] = fmaf(d[e], hat[e], dwq[e]); dbq[e] += d[e];
                         d[e] *= v[e];
-                        s1 += d[e]; s2 = fmaf(d[e], hat[e], s2);
                     }
+                    sums(d, hat, s1, s2);
                     row_sum2<WAVES>(s1, s2, lanes, sh, turn);
                     s1 = a.post == 1 ? s1 * invC : 0.f; s2 *= invC;
 #pragma unroll
@@ -190,7 +203,7 @@ __global__ __launch_bounds__(WAVES > 1 ? WAVES * 64 : 256, WAVES > 4 ? 2 : bwd_w
                     Chunk<TB> o;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) o.set(e, d[e]);
-                    store_chunk(o, at((TB*)a.db, row, a.C, dense), k);
+                    store_chunk(o, at((TB*)a.db, row, a.C, dense), a.C);
                 }
         };
         BwdRow<TX, TB, GATE == 2> r0, r1;
@@ -223,29 +236,36 @@ __global__ __launch_bounds__(WAVES > 1 ? WAVES * 64 : 256, WAVES > 4 ? 2 : bwd_w
 }
 
 // Joins the partial sums in a fixed order: workgroup row blockIdx.x < slots is a vector's gradient, the others are samples' gates.
-// 8 columns x 32 parts a workgroup, as colreduce_final_kernel.
+// 32 columns x 32 parts a workgroup, four columns a thread: whole 128-byte lines, eight of them in flight a thread (2048 columns of three
+// vectors from 1024 workgroups, 25 MB: 15.6 us with eight columns a workgroup, 6.1 us now).
 template <typename TB>
 __global__ __launch_bounds__(256) void resnorm_join_kernel(const float* __restrict__ partial, int blocks, int slots, float* __restrict__ out,
         const float* __restrict__ gate_partial, int units_per_sample, TB* __restrict__ dgate, int C) {
-    __shared__ float sh[32][9];
-    const int cx = threadIdx.x & 7, part = threadIdx.x >> 3, col = blockIdx.y * 8 + cx;
+    __shared__ float sh[32][33];
+    const int cx = (threadIdx.x & 7) * 4, part = threadIdx.x >> 3, col = blockIdx.y * 32 + cx;
     const bool vec = (int)blockIdx.x < slots;
     const int smp = (int)blockIdx.x - slots;
-    const float* p = vec ? partial + (int64_t)blockIdx.x * C : gate_partial + (int64_t)smp * units_per_sample * C;
+    const float* p = (vec ? partial + (int64_t)blockIdx.x * C : gate_partial + (int64_t)smp * units_per_sample * C) + col;
     const int64_t step = vec ? (int64_t)slots * C : C;
-    const int count = vec ? blocks : units_per_sample;
-    float s = 0.f;
-    if (col < C) {
-#pragma unroll 4
-        for (int i = part; i < count; i += 32) s += p[(int64_t)i * step + col];
+    const int count = vec ? blocks : units_per_sample, n = C - col;
+    floatx4 s = {0.f, 0.f, 0.f, 0.f};
+    if (n >= 4) {
+#pragma unroll 8
+        for (int i = part; i < count; i += 32) s += ((const Fl4u*)(p + (int64_t)i * step))->v;
+    } else if (n > 0) {
+        for (int i = part; i < count; i += 32)
+#pragma unroll
+            for (int e = 0; e < 3; ++e) if (e < n) s[e] += p[(int64_t)i * step + e];
     }
-    sh[part][cx] = s;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sh[part][cx + e] = s[e];
     __syncthreads();
-    if (part == 0 && col < C) {
+    const int mine = blockIdx.y * 32 + (int)threadIdx.x;
+    if (threadIdx.x < 32 && mine < C) {
         float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) t += sh[i][cx];
-        if (vec) out[(int64_t)blockIdx.x * C + col] = t; else dgate[(int64_t)smp * C + col] = from_f<TB>(t);
+        for (int i = 0; i < 32; ++i) t += sh[i][threadIdx.x];
+        if (vec) out[(int64_t)blockIdx.x * C + mine] = t; else dgate[(int64_t)smp * C + mine] = from_f<TB>(t);
     }
 }
 
@@ -307,6 +327,7 @@ extern "C" int ss_resnorm_bwd(int x_dtype, int b_dtype, const void* dh, int64_t 
     a.scale = scale; a.keep = keep; a.pre_w = pre_w; a.partial = workspace; a.gate_partial = gate_mode == 1 && p.units_per_sample > 1 ? workspace + (int64_t)p.blocks * p.slots * C : nullptr;
     a.lddh = (int)lddh; a.lddy = (int)lddy; a.ldh = (int)ldh; a.ldb = (int)ldb; a.ldg = (int)ldg; a.sample_rows = (int)p.sample_rows;
     a.per_sample = fast_div((unsigned)rows_per_sample); a.units = p.units; a.units_per_sample = p.units_per_sample; a.slots = p.slots;
+    a.ragged = C % 8 ? 2 : C != (p.waves > 1 ? p.waves * 64 : p.lpr) * 8;
     a.C = C; a.lpr = p.lpr; a.post = post; a.pre = pre; a.gate_mode = gate_mode; a.act = act; a.alpha = alpha;
     const size_t shm = (size_t)4 * (p.waves > 1 ? p.waves * 64 : p.lpr) * 8 * sizeof(float);
 #define SS_RN_L(TX, TB, W, P, G) hipLaunchKernelGGL((resnorm_bwd_kernel<TX, TB, W, P, G>), dim3((unsigned)p.blocks), dim3(W > 1 ? W * 64 : 256), shm, stream, a)
@@ -319,7 +340,7 @@ extern "C" int ss_resnorm_bwd(int x_dtype, int b_dtype, const void* dh, int64_t 
     SS_LAUNCH_CHECK();
     const int64_t join = p.slots + (a.gate_partial ? rows / rows_per_sample : 0);
     if (join > 0) {
-        const dim3 grid((unsigned)join, (unsigned)cdiv(C, 8));
+        const dim3 grid((unsigned)join, (unsigned)cdiv(C, 32));
         if (b_dtype == SS_BF16) hipLaunchKernelGGL(resnorm_join_kernel<bf16>, grid, dim3(256), 0, stream, workspace, p.blocks, p.slots, dvec,
                                                    a.gate_partial, p.units_per_sample, (bf16*)dgate, C);
         else hipLaunchKernelGGL(resnorm_join_kernel<float>, grid, dim3(256), 0, stream, workspace, p.blocks, p.slots, dvec, a.gate_partial,
