@@ -86,6 +86,25 @@ def _load():
     return _lib
 
 
+_native = None
+
+
+def native():
+    """the C++ host module (csrc/native.cpp), working on the library that lib() loads; no fallback path"""
+    global _native
+    if _native is None:
+        handle = _load()                                # torch and the library first
+        try:
+            from . import _native as module
+        except ImportError as e:
+            raise RuntimeError(f'semseg_amd/_native.so does not load ({e}): run `python -c "import __graft_entry__ as g; g.build()"` '
+                               '(semseg_amd has no fallback path)') from e
+        module.init(*(ctypes.cast(getattr(handle, n), ctypes.c_void_p).value
+                      for n in ('ss_resnorm_fwd', 'ss_resnorm_bwd_workspace', 'ss_resnorm_bwd', 'ss_last_error')))
+        _native = module
+    return _native
+
+
 def check(rc):
     if rc != 0:
         raise RuntimeError(f'semseg_hip error {rc}: {lib().ss_last_error().decode()}')

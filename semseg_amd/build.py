@@ -1,4 +1,5 @@
-"""Builds semseg_amd/libsemseg_hip.so (gfx950 only) from semseg_amd/csrc/*.hip with hipcc, in-tree."""
+"""Builds semseg_amd/libsemseg_hip.so (gfx950 only) from semseg_amd/csrc/*.hip with hipcc, and semseg_amd/_native.so (host code: the autograd
+node and lists whose cost is the host's) from csrc/native.cpp, both in-tree."""
 import os
 import subprocess
 import sys
@@ -12,6 +13,21 @@ LIB = os.path.join(HERE, 'libsemseg_hip.so')
 # no packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on gfx950
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=fast-honor-pragmas', '-Wno-unused-result',
          '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+
+
+NATIVE = os.path.join(HERE, '_native.so')
+
+
+def native_command():
+    """csrc/native.cpp -> _native.so: host code against torch's headers (no device code)"""
+    import sysconfig
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    root = os.path.dirname(torch.__file__)
+    inc = [f for p in include_paths() + ['/opt/rocm/include'] for f in ('-isystem', p)] + ['-I' + sysconfig.get_paths()['include']]
+    return ['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM',
+            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}'] + inc + [os.path.join(CSRC, 'native.cpp'), '-o', NATIVE,
+            '-L' + os.path.join(root, 'lib'), '-ltorch', '-ltorch_cpu', '-ltorch_hip', '-lc10', '-lc10_hip', '-ltorch_python']
 
 
 def _newer(src, dst, deps):
@@ -32,19 +48,25 @@ def build(force=False, verbose=True):
         if force or _newer(src, obj, hdrs):
             jobs.append((src, obj))
 
+    native = os.path.join(CSRC, 'native.cpp')
+
     def cc(job):
         src, obj = job
-        r = subprocess.run([hipcc] + FLAGS + ['-c', src, '-o', obj], capture_output=True, text=True)
+        cmd = native_command() if src == native else [hipcc] + FLAGS + ['-c', src, '-o', obj]
+        r = subprocess.run(cmd, capture_output=True, text=True)
         return src, r.returncode, r.stderr
 
+    device_jobs = bool(jobs)
+    if force or _newer(native, NATIVE, []):
+        jobs.append((native, NATIVE))
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
         for src, rc, err in ex.map(cc, jobs):
             if verbose:
-                print(f'[build] hipcc {os.path.basename(src)} -> rc {rc}')
+                print(f'[build] {os.path.basename(src)} -> rc {rc}')
             if rc != 0:
-                raise RuntimeError(f'hipcc failed for {src}:\n{err}')
+                raise RuntimeError(f'compiling {src} failed:\n{err}')
     objs = [os.path.join(OBJ, s[:-4] + '.o') for s in srcs]
-    if force or jobs or not os.path.exists(LIB):
+    if force or device_jobs or not os.path.exists(LIB):
         r = subprocess.run([hipcc, '--offload-arch=gfx950', '-shared', '-fPIC', '-o', LIB] + objs, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError('link failed:\n' + r.stderr)

@@ -20,7 +20,7 @@ import torch
 import torch.distributed as dist
 
 from . import ops, weightprep
-from ._lib import lib, check
+from ._lib import lib, check, native
 
 
 def _world():
@@ -396,25 +396,12 @@ class AdamW:
         self._lr_dev.copy_(torch.tensor(self._pushed, dtype=torch.float64))
 
     def _addresses(self):
-        """-> gradient type, HOST arrays of the parameters' and gradients' addresses.  Whole-list passes over bound methods: a loop with the
-        same checks takes twice as long, and a step over 200 small tensors is host time."""
+        """-> code of the gradients' type, HOST arrays of the parameters' and gradients' addresses (checked in C++: in Python the checks of a
+        few hundred tensors cost more than their step)"""
         if self.flat is not None:
             f = self.flat
-            return torch.float32, array.array('Q', (f.data.data_ptr(),)), array.array('Q', (f.grad.data_ptr(),))
-        T, ps = torch.Tensor, self.params
-        if list(map(T.numel, ps)) != self.numels or {p.dtype for p in ps} != {self.dtype} or set(map(T.get_device, ps)) != {self.device.index} \
-                or not all(map(T.is_contiguous, ps)):
-            raise RuntimeError('AdamW: a parameter changed its type, device, size or layout')
-        pa = array.array('Q', map(T.data_ptr, ps))
-        grads = [p.grad for p in ps]
-        there = [g for g in grads if g is not None]
-        types = {g.dtype for g in there}
-        if len(types) > 1 or types - {torch.float32, torch.bfloat16} or not all(map(T.is_contiguous, there)) \
-                or set(map(T.get_device, there)) - {self.device.index} \
-                or list(map(T.numel, there)) != (self.numels if len(there) == len(ps) else [n for n, g in zip(self.numels, grads) if g is not None]):
-            raise RuntimeError('AdamW: gradients must be contiguous, of one type (float32 or bfloat16) and like their parameters')
-        ga = array.array('Q', map(T.data_ptr, there) if len(there) == len(ps) else (0 if g is None else g.data_ptr() for g in grads))
-        return types.pop() if types else torch.float32, pa, ga
+            return 0, f.data.data_ptr().to_bytes(8, 'little'), f.grad.data_ptr().to_bytes(8, 'little')
+        return native().addresses(self.params, self.numels, ops._DT[self.dtype], self.device.index)
 
     def step(self, grad_scale=1.0):
         if self.device.type != 'cuda':
@@ -424,8 +411,7 @@ class AdamW:
             raise RuntimeError('AdamW.step: captured into a graph it would repeat one step for ever; build it with capturable=True')
         if self.capturable and not capturing and self._rates() != self._pushed:
             self.push_lr()
-        gt, p_list, g_list = self._addresses()
-        pa, ga = p_list.buffer_info()[0], g_list.buffer_info()[0]
+        gt, pa, ga = self._addresses()
         plan, norm, k = self.plan, None, len(self.groups)
         lr = array.array('d', [self.lr * r for r, _ in self.groups])
         wd = array.array('d', [self.wd if w is None else w for _, w in self.groups])
@@ -434,7 +420,7 @@ class AdamW:
             measured = self.max_grad_norm is not None or self.skip_nonfinite
             if self._t_dev is None:
                 self._t += 1
-            args = (ops._DT[self.dtype], ops._DT[gt], self.state_bits, plan.count, pa, ga, plan.first_chunk, plan.table.data_ptr(), self.exp_avg.data_ptr(),
+            args = (ops._DT[self.dtype], gt, self.state_bits, plan.count, pa, ga, plan.first_chunk, plan.table.data_ptr(), self.exp_avg.data_ptr(),
                     self.exp_avg_sq.data_ptr(), ops._p(self.exp_avg_scale), ops._p(self.exp_avg_sq_scale), b1, b2, self.eps, grad_scale, self._t, k,
                     lr.buffer_info()[0], wd.buffer_info()[0], self.seed)
             if measured or self._t_dev is not None:

@@ -12,7 +12,7 @@ parameters are fp32.  ``y`` is the norm of ``h`` as it is stored, so that it is 
 import torch
 from torch import nn, Tensor
 
-from . import ops
+from . import _lib, ops
 from .runtime import GradAwareFunction, deliver_grads, drop_path_keep, expect_grads
 
 _VECTORS = ('pre_w', 'pre_b', 'post_w', 'post_b', 'scale')
@@ -78,6 +78,15 @@ def gated_residual_norm(x: Tensor, branch: Tensor, *, post='none', post_weight=N
     (weight, optionally bias) or 'rms' (weight).  gate (branch's type): per sample [samples, C] or per element, shaped like x; gate_act:
     'none' or 'sigmoid'.  scale, weights, biases: float32 [C].  keep: float32 [samples].  A sample is an index of x's first dimension (a 2-D
     x is one sample) unless ``samples`` says into how many equal runs of rows x divides.  Differentiable in everything but keep."""
+    if _lib.TRACE is None and not (torch.is_grad_enabled() and any(getattr(v, '_ss_grad_sink', None) is not None
+                                                                     for v in (scale, pre_weight, post_weight, pre_bias, post_bias))):
+        if post not in ops._NORM or pre not in ops._NORM or gate_act not in ops._GATE_ACT:
+            raise ValueError(f'gated_residual_norm: unknown norm or gate activation in {post!r}, {pre!r}, {gate_act!r}')
+        if samples is not None and samples < 1:
+            raise ValueError(f'gated_residual_norm: rows do not divide into {samples} samples')
+        return _lib.native().gated_residual_norm(x, branch, ops._NORM[post], post_weight, post_bias, gate, ops._GATE_ACT[gate_act], scale, keep, alpha,
+                                                 ops._NORM[pre], pre_weight, pre_bias, eps, samples or 0)
+    # parameters with a slot in engine.FlatParams' gradient buffer, and traced calls: the same node in Python, which delivers there
     shape = x.shape
     if len(shape) < 2 or branch.shape != shape:
         raise ValueError(f'gated_residual_norm: x {tuple(shape)} and branch {tuple(branch.shape)} must be alike, [..., C]')

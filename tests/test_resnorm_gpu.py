@@ -355,3 +355,61 @@ def test_a_row_has_the_same_bits_in_any_company(C, dtype):
         part = {k: v if v is None or v.dim() == 1 else v[lo:hi] for k, v in d.items()}
         h1, y1, st1 = ops.resnorm_fwd(**part, **dict(meta, rows_per_sample=hi - lo))
         assert torch.equal(h1, h[lo:hi]) and torch.equal(y1, y[lo:hi]) and torch.equal(st1, st[lo:hi])
+
+
+@pytest.mark.parametrize('post,pre,gate,act,keep', [('layer', 'layer', 'sample', 'sigmoid', True), ('rms', 'none', 'row', 'none', False),
+                                                    ('none', 'layer', 'none', 'none', True), ('none', 'none', 'none', 'none', False)])
+def test_both_nodes_agree_bit_for_bit(post, pre, gate, act, keep):
+    """the C++ node, and the Python one that parameters of engine.FlatParams and traced calls take"""
+    from semseg_amd import _lib
+    from semseg_amd.resnorm import gated_residual_norm
+    t, meta, dh, dy = make(60, 72, F, H, seed=3, samples=4, post=post, pre=pre, gate=gate, act=act, keep=keep, alpha=0.5)
+
+    def run():
+        L = _leaves(t)
+        view = {k: v.view(4, 15, 72) if k in 'xb' or (k == 'gate' and gate == 'row') else v for k, v in L.items()}
+        h, y = gated_residual_norm(view['x'], view['b'], post=post, post_weight=L.get('post_w'), post_bias=L.get('post_b'), gate=view.get('gate'),
+                                   gate_act=act, scale=L['scale'], keep=L.get('keep'), alpha=0.5, pre=pre, pre_weight=L.get('pre_w'), pre_bias=L.get('pre_b'))
+        outs, grads = ([h, y], [dh.cuda().view(4, 15, 72), dy.cuda().view(4, 15, 72)]) if y is not None else ([h], [dh.cuda().view(4, 15, 72)])
+        names = [k for k in L if k != 'keep']
+        return outs + list(torch.autograd.grad(outs, [L[k] for k in names], grads))
+    native = run()
+    _lib.TRACE = []
+    try:
+        python = run()
+        assert {e[0] for e in _lib.TRACE} == {'ss_resnorm_fwd', 'ss_resnorm_bwd'}
+    finally:
+        _lib.TRACE = None
+    assert len(native) == len(python) and all(torch.equal(a, b) for a, b in zip(native, python))
+
+
+def test_parameters_of_other_shapes_and_flat_parameters():
+    """a vector shaped [1, C] gets its gradient in that shape; parameters in FlatParams' buffer find theirs there, added to what is there"""
+    from semseg_amd.engine import FlatParams
+    from semseg_amd.resnorm import GatedResidualNorm, gated_residual_norm
+    torch.manual_seed(0)
+    x, b = torch.randn(5, 40, device='cuda'), torch.randn(5, 40, device='cuda')
+    w = torch.rand(1, 40, device='cuda', requires_grad=True)
+    h, y = gated_residual_norm(x, b, pre='rms', pre_weight=w)
+    y.sum().backward()
+    flat_w = w.detach().view(40).clone().requires_grad_()
+    gated_residual_norm(x, b, pre='rms', pre_weight=flat_w)[1].sum().backward()
+    assert w.grad.shape == (1, 40) and torch.equal(w.grad.view(40), flat_w.grad)
+    a, c = (GatedResidualNorm(40, post='rms', layer_scale=0.3).cuda() for _ in range(2))
+    flat = FlatParams(c)
+    for m in (a, c):
+        for _ in range(2):                                     # gradients accumulate
+            h, y = m(x.view(1, 5, 40), b.view(1, 5, 40))
+            (h.sum() + (y * y).sum()).backward()
+    for p, q in zip(a.parameters(), c.parameters()):
+        assert torch.equal(p.grad, q.grad) and q.grad.data_ptr() >= flat.grad.data_ptr()
+
+
+def test_leaves_changed_in_place_before_backward_are_noticed():
+    from semseg_amd.resnorm import GatedResidualNorm
+    m = GatedResidualNorm(16).cuda()
+    x, b = torch.randn(2, 3, 16, device='cuda', requires_grad=True), torch.randn(2, 3, 16, device='cuda')
+    h, y = m(x, b)
+    b.mul_(2.0)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
