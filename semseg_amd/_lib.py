@@ -100,7 +100,7 @@ def native():
             raise RuntimeError(f'semseg_amd/_native.so does not load ({e}): run `python -c "import __graft_entry__ as g; g.build()"` '
                                '(semseg_amd has no fallback path)') from e
         module.init(*(ctypes.cast(getattr(handle, n), ctypes.c_void_p).value
-                      for n in ('ss_resnorm_fwd', 'ss_resnorm_bwd_workspace', 'ss_resnorm_bwd', 'ss_last_error')))
+                      for n in ('ss_resnorm_fwd', 'ss_resnorm_bwd_workspace', 'ss_resnorm_bwd', 'ss_multi_add_f32', 'ss_last_error')))
         _native = module
     return _native
 

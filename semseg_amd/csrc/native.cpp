@@ -23,10 +23,12 @@ typedef int64_t (*ws_fn)(int64_t, int64_t, int, int, int, int, int);
 typedef int (*bwd_fn)(int, int, const void*, int64_t, const void*, int64_t, const void*, int64_t, const void*, int64_t, const void*, int64_t, int, int,
                       const float*, const float*, float, int, const float*, const float*, int, const float*, const float*, void*, void*, void*, float*, int64_t,
                       int64_t, int, float*, int64_t, void*);
+typedef int (*add_fn)(int, const float* const*, const int64_t*, const int64_t*, float* const*, const int64_t*, void*);
 typedef const char* (*err_fn)();
 fwd_fn resnorm_fwd = nullptr;
 ws_fn resnorm_ws = nullptr;
 bwd_fn resnorm_bwd = nullptr;
+add_fn multi_add = nullptr;
 err_fn last_error = nullptr;
 
 void check(int rc) { TORCH_CHECK(rc == 0, "semseg_hip error ", rc, ": ", last_error()); }
@@ -38,7 +40,8 @@ std::string str(c10::IntArrayRef s) {
     return r + ")";
 }
 
-struct Cfg { int64_t rows, n, C; int mode, post, pre, act; double alpha, eps; };
+// sinks: the vectors' slots in a flat gradient buffer (engine.FlatParams), undefined where there is none
+struct Cfg { int64_t rows, n, C; int mode, post, pre, act; double alpha, eps; std::vector<Tensor> sinks; };
 int code(const Tensor& t) { return t.scalar_type() == at::kBFloat16; }
 const float* f32(const Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
 const void* raw(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
@@ -74,6 +77,25 @@ Forward launch_forward(const Tensor& x, const Tensor& b, const Tensor& gate, con
 typedef std::optional<Tensor> Maybe;
 Tensor or_none(const Maybe& t) { return t ? *t : Tensor(); }
 
+// What runtime.deliver_grads does: gradients whose parameter still has its slot as .grad are added there, all in one launch, and autograd is
+// handed nothing for them.
+void deliver(const std::vector<Tensor>& sinks, const variable_list& params, variable_list& out, void* stream) {
+    const float* src[5];
+    float* dst[5];
+    int64_t n[5];
+    int k = 0;
+    for (int i = 0; i < 5; ++i) {
+        Tensor& g = out[4 + i];
+        if (!g.defined() || !sinks[i].defined() || !params[i].grad().defined() || params[i].grad().const_data_ptr() != sinks[i].const_data_ptr() ||
+            sinks[i].numel() != g.numel() || !params[i].requires_grad()) continue;
+        src[k] = g.const_data_ptr<float>(); dst[k] = sinks[i].mutable_data_ptr<float>(); n[k] = g.numel();
+        ++k;
+    }
+    if (k) check(multi_add(k, src, n, n, dst, n, stream));
+    for (int i = 0, j = 0; i < 5 && j < k; ++i)                              // the launch has read them: the allocator keeps stream order
+        if (out[4 + i].defined() && out[4 + i].const_data_ptr<float>() == src[j]) { out[4 + i] = Tensor(); ++j; }
+}
+
 // Inputs: x, branch, gate, keep, then the vectors: pre weight, pre bias, post weight, post bias, scale
 struct ResnormNode : public torch::autograd::Function<ResnormNode> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& b, const Maybe& gate_, const Maybe& keep_, const Maybe& pre_w_,
@@ -86,6 +108,7 @@ struct ResnormNode : public torch::autograd::Function<ResnormNode> {
         auto& s = ctx->saved_data;
         s["i"] = std::vector<int64_t>{c.rows, c.n, c.C, c.mode, c.post, c.pre, c.act};
         s["alpha"] = c.alpha;
+        if (!c.sinks.empty()) s["sinks"] = c.sinks;
         if (c.pre) return {r.h, r.y};
         return {r.h};
     }
@@ -125,20 +148,22 @@ struct ResnormNode : public torch::autograd::Function<ResnormNode> {
         if (post) out[6] = slot(post_w);
         if (post == 1) { const Tensor t = slot(post_b); if (post_b.defined()) out[7] = t; }
         if (has_scale) out[8] = slot(scale);
+        if (ctx->saved_data.count("sinks")) deliver(ctx->saved_data["sinks"].toTensorVector(), {pre_w, saved[6], post_w, post_b, scale}, out, stream_of(h));
         return out;
     }
 };
 
 py::object gated_residual_norm(const Tensor& x, const Tensor& branch, int post, const Maybe& post_w_, const Maybe& post_b_, const Maybe& gate_, int act,
                                const Maybe& scale_, const Maybe& keep_, double alpha, int pre, const Maybe& pre_w_, const Maybe& pre_b_, double eps,
-                               int64_t samples) {
+                               int64_t samples, const std::vector<Maybe>& sinks) {
     const Tensor post_w = or_none(post_w_), post_b = or_none(post_b_), gate = or_none(gate_), scale = or_none(scale_), keep = or_none(keep_),
                  pre_w = or_none(pre_w_), pre_b = or_none(pre_b_);
     typedef py::value_error Value;
     typedef py::type_error Type;
     if (x.dim() < 2 || !x.sizes().equals(branch.sizes()))
         fail<Value>("x " + str(x.sizes()) + " and branch " + str(branch.sizes()) + " must be alike, [..., C]");
-    Cfg c{0, 0, x.size(-1), 0, post, pre, act, alpha, eps};
+    Cfg c{0, 0, x.size(-1), 0, post, pre, act, alpha, eps, {}};
+    for (const Maybe& t : sinks) c.sinks.push_back(or_none(t));
     if (x.numel() == 0) fail<Value>("nothing in x " + str(x.sizes()));
     c.rows = x.numel() / c.C;
     if (samples == 0) samples = x.dim() > 2 ? x.size(0) : 1;
@@ -206,10 +231,11 @@ py::tuple addresses(const std::vector<Tensor>& params, const std::vector<int64_t
     return py::make_tuple(gt < 0 ? 0 : gt, py::bytes((const char*)pa.data(), pa.size() * 8), py::bytes((const char*)ga.data(), ga.size() * 8));
 }
 
-void init(uint64_t fwd, uint64_t ws, uint64_t bwd, uint64_t err) {
+void init(uint64_t fwd, uint64_t ws, uint64_t bwd, uint64_t add, uint64_t err) {
     resnorm_fwd = (fwd_fn)fwd;
     resnorm_ws = (ws_fn)ws;
     resnorm_bwd = (bwd_fn)bwd;
+    multi_add = (add_fn)add;
     last_error = (err_fn)err;
 }
 

@@ -78,15 +78,17 @@ def gated_residual_norm(x: Tensor, branch: Tensor, *, post='none', post_weight=N
     (weight, optionally bias) or 'rms' (weight).  gate (branch's type): per sample [samples, C] or per element, shaped like x; gate_act:
     'none' or 'sigmoid'.  scale, weights, biases: float32 [C].  keep: float32 [samples].  A sample is an index of x's first dimension (a 2-D
     x is one sample) unless ``samples`` says into how many equal runs of rows x divides.  Differentiable in everything but keep."""
-    if _lib.TRACE is None and not (torch.is_grad_enabled() and any(getattr(v, '_ss_grad_sink', None) is not None
-                                                                     for v in (scale, pre_weight, post_weight, pre_bias, post_bias))):
+    vectors = (pre_weight, pre_bias, post_weight, post_bias, scale)
+    if _lib.TRACE is None and not any(hasattr(v, '_ss_grad_ready') for v in vectors):
         if post not in ops._NORM or pre not in ops._NORM or gate_act not in ops._GATE_ACT:
             raise ValueError(f'gated_residual_norm: unknown norm or gate activation in {post!r}, {pre!r}, {gate_act!r}')
         if samples is not None and samples < 1:
             raise ValueError(f'gated_residual_norm: rows do not divide into {samples} samples')
+        sinks = [getattr(v, '_ss_grad_sink', None) for v in vectors]            # slots in engine.FlatParams' gradient buffer
         return _lib.native().gated_residual_norm(x, branch, ops._NORM[post], post_weight, post_bias, gate, ops._GATE_ACT[gate_act], scale, keep, alpha,
-                                                 ops._NORM[pre], pre_weight, pre_bias, eps, samples or 0)
-    # parameters with a slot in engine.FlatParams' gradient buffer, and traced calls: the same node in Python, which delivers there
+                                                 ops._NORM[pre], pre_weight, pre_bias, eps, samples or 0,
+                                                 sinks if any(s is not None for s in sinks) else [])
+    # parameters whose gradients an engine.GradReducer waits for (its callbacks are Python), and traced calls: the same node in Python
     shape = x.shape
     if len(shape) < 2 or branch.shape != shape:
         raise ValueError(f'gated_residual_norm: x {tuple(shape)} and branch {tuple(branch.shape)} must be alike, [..., C]')
@@ -110,7 +112,6 @@ def gated_residual_norm(x: Tensor, branch: Tensor, *, post='none', post_weight=N
         raise TypeError(f'gated_residual_norm: stream / branch types must be f32 / f32, bf16 / bf16 or f32 / bf16, got {x.dtype} / {branch.dtype}')
     post_k, pre_k, act = ops._resnorm_vectors(C, samples, device, gate_act, scale, keep, post, post_weight, post_bias, pre, pre_weight, pre_bias,
                                               'gated_residual_norm')
-    vectors = (pre_weight, pre_bias, post_weight, post_bias, scale)
     if torch.is_grad_enabled() and (x.requires_grad or branch.requires_grad or (mode and gate.requires_grad) or
                                     any(t is not None and t.requires_grad for t in vectors)):
         return _ResnormFn.apply(x, branch, gate, keep, (rows, rows // samples, C, mode, post_k, pre_k, act, float(alpha), float(eps)), *vectors)

@@ -413,3 +413,37 @@ def test_leaves_changed_in_place_before_backward_are_noticed():
     b.mul_(2.0)
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
         y.sum().backward()
+
+
+def test_flat_parameters_with_a_reducer_take_the_python_node():
+    """a GradReducer's callbacks are counted as for every other node (one process: the reducer is made active by hand)"""
+    from semseg_amd.engine import FlatParams
+    from semseg_amd.resnorm import GatedResidualNorm
+    torch.manual_seed(1)
+    a, c = (GatedResidualNorm(24, post='layer', layer_scale=0.3).cuda() for _ in range(2))
+    FlatParams(a), FlatParams(c)
+    seen = []
+    for p in c.parameters():
+        p._ss_grad_ready = lambda q: seen.append(q)
+    x, b = torch.randn(2, 5, 24, device='cuda'), torch.randn(2, 5, 24, device='cuda')
+    for m in (a, c):
+        h, y = m(x, b)
+        (h.sum() + (y * y).sum()).backward()
+    assert len(seen) == 5 and {id(p) for p in seen} == {id(p) for p in c.parameters()}
+    assert all(torch.equal(p.grad, q.grad) for p, q in zip(a.parameters(), c.parameters()))
+
+
+def test_frozen_flat_parameters_and_replaced_gradients():
+    from semseg_amd.engine import FlatParams
+    from semseg_amd.resnorm import GatedResidualNorm
+    torch.manual_seed(2)
+    m = GatedResidualNorm(24, post='rms', layer_scale=0.3).cuda()
+    flat = FlatParams(m)
+    m.pre_weight.requires_grad_(False)                         # frozen after the buffer was laid out: its slot stays zero
+    slot = m.scale.grad
+    m.scale.grad = torch.zeros(24, device='cuda')              # no longer the slot: the gradient goes to what .grad is
+    x, b = torch.randn(2, 5, 24, device='cuda'), torch.randn(2, 5, 24, device='cuda')
+    h, y = m(x, b)
+    (h.sum() + (y * y).sum()).backward()
+    assert (m.pre_weight.grad == 0).all() and (slot == 0).all() and (m.scale.grad != 0).any() and (m.post_weight.grad != 0).any()
+    assert m.post_weight.grad.data_ptr() >= flat.grad.data_ptr()
