@@ -127,12 +127,12 @@ __device__ __forceinline__ float clip_coef(double norm, double max_norm, double 
     return (float)(clip * grad_scale);
 }
 // What the gradients are multiplied by: made by adamw_prepare_kernel, joined here, or given
-__device__ __forceinline__ float step_coef(const AdamArgs& a, const AdamDyn* __restrict__ dyn, bool writes) {
+__device__ __forceinline__ float step_coef(const AdamArgs& a, const AdamDyn* __restrict__ dyn) {
     if (dyn) return dyn->coef;
     if (!a.partial) return a.dyn.coef;
     __shared__ double sh[4];
     const double norm = sqrt(join_sums(a.partial, a.sums, sh)) * a.grad_scale;
-    if (writes && a.norm && threadIdx.x == 0) *a.norm = (float)norm;
+    if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = (float)norm;
     return clip_coef(norm, a.max_norm, a.grad_scale);
 }
 
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamPtrs2 ptrs, const Adam
         float* __restrict__ v, AdamArgs a, const AdamDyn* __restrict__ dyn) {
     if (dyn && dyn->skip) return;
     const AdamChunk c = plan[blockIdx.x];
-    const float coef = step_coef(a, dyn, first_tensor == 0 && blockIdx.x == 0), rbc2 = dyn ? dyn->rbc2 : a.dyn.rbc2;
+    const float coef = step_coef(a, dyn), rbc2 = dyn ? dyn->rbc2 : a.dyn.rbc2;
     const float step = dyn ? dyn->step[c.group] : a.dyn.step[c.group], decay = dyn ? dyn->decay[c.group] : a.dyn.decay[c.group];
     const TG* __restrict__ g = (const TG*)ptrs.g[c.tensor - first_tensor];
     if (!g) return;                                            // no gradient: the tensor and its moments stay
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamPtrs2 ptrs, const AdamC
         unsigned* __restrict__ vc, float* __restrict__ qm, float* __restrict__ qv, AdamArgs a, const AdamDyn* __restrict__ dyn) {
     if (dyn && dyn->skip) return;
     const AdamChunk c = plan[blockIdx.x];
-    const float coef = step_coef(a, dyn, first_tensor == 0 && blockIdx.x == 0), rbc2 = dyn ? dyn->rbc2 : a.dyn.rbc2;
+    const float coef = step_coef(a, dyn), rbc2 = dyn ? dyn->rbc2 : a.dyn.rbc2;
     const float step = dyn ? dyn->step[c.group] : a.dyn.step[c.group], decay = dyn ? dyn->decay[c.group] : a.dyn.decay[c.group];
     const unsigned key = dyn ? dyn->key : a.dyn.key;
     const TG* __restrict__ g = (const TG*)ptrs.g[c.tensor - first_tensor];
@@ -422,6 +422,7 @@ static int adamw_step(int p_dtype, int g_dtype, int bits, int count, void* const
         else { if (g_dtype == SS_F32) SS_ADAMW(bf16, float); else SS_ADAMW(bf16, bf16); }
 #undef SS_ADAMW
         SS_LAUNCH_CHECK();
+        a.norm = nullptr;                                      // the first launch has written it
     }
     return 0;
 }

@@ -7,6 +7,9 @@
 #include <torch/extension.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/graph_task.h>
 
 #include <string>
 #include <vector>
@@ -47,14 +50,15 @@ const float* f32(const Tensor& t) { return t.defined() ? t.const_data_ptr<float>
 const void* raw(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
 
-// [..., C] with unit inner stride and one stride between rows; a view or a copy only where the layout asks for one
+// [..., C] with unit inner stride and one stride between rows that the kernels' 32-bit lane offsets reach; a view or a copy only where the
+// layout asks for one
 Tensor rows_of(const Tensor& t, int64_t C, int64_t& ld) {
     ld = 0;
     if (!t.defined()) return t;
     ld = C;
     if (t.is_contiguous()) return t;
     Tensor r = t.dim() == 2 ? t : t.reshape({-1, C});
-    if (r.stride(1) != 1) return r.contiguous();
+    if (r.stride(1) != 1 || r.stride(0) >= (1 << 23)) return r.contiguous();
     ld = r.stride(0);
     return r;
 }
@@ -96,6 +100,25 @@ void deliver(const std::vector<Tensor>& sinks, const variable_list& params, vari
         if (out[4 + i].defined() && out[4 + i].const_data_ptr<float>() == src[j]) { out[4 + i] = Tensor(); ++j; }
 }
 
+// A leaf's gradient is handed over on the stream on which the oldest living graph used the leaf.  In a capture that must not be the default
+// stream: the capture cannot take its work in, and the process ends over it.  So such a backward is refused before it gets there.
+void refuse_default_stream_leaves() {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto node = torch::autograd::get_current_node();
+    const auto* info = torch::autograd::get_current_graph_task_exec_info();
+    for (const auto& edge : node->next_edges()) {
+        auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
+        if (!leaf) continue;
+        if (info && !info->empty()) {                                        // autograd.grad: only what is asked for; it goes to the leaf's stream too
+            const auto it = info->find(leaf);
+            if (it == info->end() || !it->second.should_execute()) continue;
+        }
+        const auto s = leaf->stream();
+        TORCH_CHECK(!s || s->id() != 0, "gated_residual_norm: backward captured while an eager graph of the same leaves, made on the default stream, is alive; "
+                    "drop its outputs first, or run the eager passes on a side stream");
+    }
+}
+
 // Inputs: x, branch, gate, keep, then the vectors: pre weight, pre bias, post weight, post bias, scale
 struct ResnormNode : public torch::autograd::Function<ResnormNode> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& b, const Maybe& gate_, const Maybe& keep_, const Maybe& pre_w_,
@@ -118,6 +141,7 @@ struct ResnormNode : public torch::autograd::Function<ResnormNode> {
         variable_list out(10);
         const Tensor dh = grads[0], dy = grads.size() > 1 ? grads[1] : Tensor();
         if (!dh.defined() && !dy.defined()) return out;
+        refuse_default_stream_leaves();
         const auto saved = ctx->get_saved_variables();
         const Tensor &h = saved[0], &b = saved[1], &gate = saved[2], &keep = saved[3], &stats = saved[4], &pre_w = saved[5], &post_w = saved[7], &post_b = saved[8],
                      &scale = saved[9];

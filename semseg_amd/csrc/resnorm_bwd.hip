@@ -103,9 +103,13 @@ __global__ __launch_bounds__(WAVES > 1 ? WAVES * 64 : 256, WAVES > 4 ? 2 : bwd_w
             const int row = begin + wave_first + i;
             const bool there = row + lr < end, ok = there && k.lo < k.hi;
             const unsigned dense = (unsigned)(lr * a.C + k.cb);
-            if (row + rpw > end) {                                           // a lane without a row adds nothing to the columns
+            if (row + rpw > end && !there) {                                 // a lane without a row adds nothing to the columns, infinities neither
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { t.dy.set(e, there ? t.dy.get(e) : 0.f); t.dh.set(e, there ? t.dh.get(e) : 0.f); }
+                for (int e = 0; e < 8; ++e) {
+                    t.dy.set(e, 0.f); t.dh.set(e, 0.f); t.h.set(e, 0.f); t.b.set(e, 0.f);
+                    if constexpr (GATE == 2) t.g[0].set(e, 0.f);
+                }
+                t.st = floatx4{0.f, 0.f, 0.f, 0.f};
             }
                 float d[8], hat[8], v[8];
                 if (a.has_dh) {

@@ -337,9 +337,12 @@ class AdamW:
                 raise ValueError('AdamW: parameters must be contiguous, of one type (float32 or bfloat16) and on one device')
         if len({id(p) for p in self.params}) != len(self.params):
             raise ValueError('AdamW: a parameter appears twice')
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
+        if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
+            raise ValueError('AdamW: parameters share memory')
         if state_bits not in (8, 32):
             raise ValueError(f'AdamW: state_bits must be 8 or 32, got {state_bits}')
-        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0) or lr < 0.0 or eps < 0.0 or weight_decay < 0.0:
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and lr >= 0.0 and eps >= 0.0 and weight_decay >= 0.0):
             raise ValueError('AdamW: betas must lie in [0, 1), lr, eps and weight_decay must not be negative')
         if max_grad_norm is not None and not max_grad_norm > 0.0:
             raise ValueError('AdamW: max_grad_norm must be positive, or None')
@@ -352,6 +355,8 @@ class AdamW:
             if set(own) - {'lr_scale', 'weight_decay'}:
                 raise ValueError(f'AdamW: per_param knows lr_scale and weight_decay, got {sorted(own)}')
             key = (float(own.get('lr_scale', 1.0)), own.get('weight_decay'))
+            if not (key[0] >= 0.0 and (key[1] is None or key[1] >= 0.0)):
+                raise ValueError(f'AdamW: lr_scale and weight_decay must not be negative, got {own}')
             if key not in self.groups:
                 self.groups.append(key)
             of.append(self.groups.index(key))
@@ -418,10 +423,8 @@ class AdamW:
         b1, b2 = self.betas
         with ops._DeviceGuard(self.device) as stream:
             measured = self.max_grad_norm is not None or self.skip_nonfinite
-            if self._t_dev is None:
-                self._t += 1
             args = (ops._DT[self.dtype], gt, self.state_bits, plan.count, pa, ga, plan.first_chunk, plan.table.data_ptr(), self.exp_avg.data_ptr(),
-                    self.exp_avg_sq.data_ptr(), ops._p(self.exp_avg_scale), ops._p(self.exp_avg_sq_scale), b1, b2, self.eps, grad_scale, self._t, k,
+                    self.exp_avg_sq.data_ptr(), ops._p(self.exp_avg_scale), ops._p(self.exp_avg_sq_scale), b1, b2, self.eps, grad_scale, self._t + 1, k,
                     lr.buffer_info()[0], wd.buffer_info()[0], self.seed)
             if measured or self._t_dev is not None:
                 # scratch from the allocator for each step: nothing that two captured steps or two streams could share
@@ -433,6 +436,8 @@ class AdamW:
                                                ops._p(norm), at + self._partial_bytes, at if measured else None, stream))
             else:
                 check(lib().ss_adamw_step(*args, None, stream))
+        if self._t_dev is None:
+            self._t += 1                                       # a step that was refused does not count
         weightprep.bump()                                      # the kernel wrote the parameters through a raw pointer
         return norm
 

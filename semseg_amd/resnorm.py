@@ -25,7 +25,7 @@ def _rows(t, C):
         return t, C
     if t.dim() != 2:
         t = t.reshape(-1, C)
-    if t.stride(1) != 1:
+    if t.stride(1) != 1 or t.stride(0) >= 1 << 23:             # 32-bit lane offsets in the kernels
         t = t.contiguous()
         return t, C
     return t, t.stride(0)

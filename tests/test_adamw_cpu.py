@@ -175,3 +175,15 @@ def test_draws_are_spread_and_independent():
         assert abs(a.mean() / 65535 - 0.5) < 4 * 0.29 / n ** 0.5 and abs(a.std() / 65535 - 12 ** -0.5) < 0.005
     for a, b in ((um, uv), (um, u2), (um, u3), (um[:, 1:], um[:, :-1]), (um[1:], um[:-1])):
         assert abs(np.corrcoef(a.ravel(), b.ravel())[0, 1]) < 5 / n ** 0.5
+
+
+def test_shared_memory_and_hyperparameters_that_are_no_numbers_are_refused():
+    from semseg_amd.engine import AdamW
+    base = torch.zeros(12)
+    with pytest.raises(ValueError, match='share memory'):
+        AdamW([base[:8], base[7:]])
+    AdamW([base[:7], base[7:], torch.zeros(0)])
+    for kw in (dict(lr=float('nan')), dict(eps=float('nan')), dict(weight_decay=-0.1), dict(per_param=lambda p: {'weight_decay': -0.1}),
+               dict(per_param=lambda p: {'lr_scale': float('nan')})):
+        with pytest.raises(ValueError, match='negative|betas'):
+            AdamW([torch.zeros(3)], **kw)

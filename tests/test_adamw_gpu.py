@@ -379,3 +379,47 @@ def test_zero_sized_and_single_element_models():
     params, opt, g = build([(0,)], seed=3, max_grad_norm=1.0)
     give(params, g, torch.float32)
     assert float(opt.step()) == 0.0 and opt.t == 1
+
+
+def test_the_norm_is_written_when_the_first_tensors_are_empty():
+    params, opt, g = build([(0,)] * 230 + [(7,)], seed=3, max_grad_norm=1.0)
+    give(params, g, torch.float32)
+    assert float(opt.step()) == pytest.approx(float(params[-1].grad.norm()), rel=1e-6)
+
+
+def test_a_refused_step_is_not_counted():
+    params, opt, g = build([(7,)], seed=3)
+    give(params, g, torch.float32)
+    before = params[0].detach().clone()
+    opt.betas = (0.9, 1.0)
+    with pytest.raises(RuntimeError, match='betas'):
+        opt.step()
+    assert opt.t == 0 and torch.equal(params[0], before)
+    opt.betas = (0.9, 0.999)
+    opt.step()
+    assert opt.t == 1 and not torch.equal(params[0], before)
+
+
+def test_elements_past_32_bits():
+    """the last elements of 2^32 + take the step that they take alone"""
+    from semseg_amd.engine import AdamW
+    n, tail = (1 << 32) + 300, 556                             # whole runs from n - 556 on
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip('needs 80 GB')
+    p = torch.full((n,), 0.5, device='cuda', dtype=torch.bfloat16)
+    p.grad = torch.full((n,), 0.25, device='cuda', dtype=torch.bfloat16)
+    q = torch.randn(tail, device='cuda').bfloat16()
+    p[-tail:].copy_(q)
+    q.grad = torch.randn(tail, device='cuda').bfloat16()
+    p.grad[-tail:].copy_(q.grad)
+    kw = dict(lr=0.05, max_grad_norm=1e9, state_bits=8)        # no clipping: every element is on its own
+    big, small = AdamW([p], **kw), AdamW([q], **kw)
+    norm = float(big.step())
+    small.step()
+    assert norm == pytest.approx(((n - tail) * 0.0625 + float((q.grad.double() ** 2).sum())) ** 0.5, rel=1e-6)
+    assert torch.equal(p[-tail:], q)
+    assert torch.equal(big.exp_avg_scale[-3:], small.exp_avg_scale) and torch.equal(big.exp_avg_sq_scale[-3:], small.exp_avg_sq_scale)
+    assert int((big.exp_avg[-768:].int() - small.exp_avg.int()).abs().max()) <= 1        # other draws, by the element's place
+    assert float(p[:1 << 20].float().std()) == 0.0 and float(p[0]) != 0.5
+    del p, big
+    torch.cuda.empty_cache()

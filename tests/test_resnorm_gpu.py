@@ -447,3 +447,129 @@ def test_frozen_flat_parameters_and_replaced_gradients():
     (h.sum() + (y * y).sum()).backward()
     assert (m.pre_weight.grad == 0).all() and (slot == 0).all() and (m.scale.grad != 0).any() and (m.post_weight.grad != 0).any()
     assert m.post_weight.grad.data_ptr() >= flat.grad.data_ptr()
+
+
+@pytest.mark.parametrize('C', [8, 64, 200])
+@pytest.mark.parametrize('rows', [1, 3, 70])
+def test_an_infinity_in_the_last_row_reaches_the_sums_as_it_is(rows, C):
+    """lanes behind the last row read that row again: they add zero, not zero times infinity"""
+    from semseg_amd import ops
+    t, meta, dh, _ = make(rows, C, F, F, seed=5)
+    d = {k: None if v is None else v.cuda() for k, v in t.items()}
+    dh = dh.cuda()
+    d['b'][-1, 3] = float('inf')
+    back = {k: v for k, v in d.items() if k not in ('x', 'b', 'pre_b')}
+    h, _, st = ops.resnorm_fwd(**d, **meta)
+    *_, G = ops.resnorm_bwd(dh, None, h, d['b'], st, **back, **meta)
+    assert G['scale'][3] == float('inf') * torch.sign(dh[-1, 3]) and torch.isfinite(torch.cat([G['scale'][:3], G['scale'][4:]])).all()
+    d['b'][-1, 3] = 1.0
+    d['gate'] = back['gate'] = torch.ones(rows, C, device='cuda')
+    d['gate'][-1, 3] = float('inf')
+    h, _, st = ops.resnorm_fwd(**d, **meta)
+    *_, G = ops.resnorm_bwd(dh, None, h, d['b'], st, **back, **meta)
+    assert G['scale'][3] == float('inf') * torch.sign(dh[-1, 3])
+
+
+def test_rows_far_apart():
+    """strides past the lanes' offsets are copied"""
+    from semseg_amd.resnorm import gated_residual_norm
+    torch.manual_seed(0)
+    x = torch.randn(3, (1 << 23) + 8, device='cuda', dtype=H)[:, :64]
+    b = torch.randn(3, 64, device='cuda', dtype=H)
+    w = torch.rand(64, device='cuda') + 0.5
+    far, near = (gated_residual_norm(v, b, pre='rms', pre_weight=w) for v in (x, x.contiguous()))
+    assert x.stride(0) > 1 << 23 and all(torch.equal(p, q) for p, q in zip(far, near))
+    grads = []
+    for dy in (x, x.contiguous()):
+        leaf = b.clone().requires_grad_()
+        _, y = gated_residual_norm(x.contiguous(), leaf, pre='rms', pre_weight=w)
+        grads += torch.autograd.grad(y, leaf, dy)
+    assert torch.equal(*grads)
+
+
+def test_offsets_past_32_bits():
+    """the last rows of 2^32 + elements have the bits that they have alone"""
+    from semseg_amd import ops
+    C, rows = 4096, (1 << 20) + 5
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip('needs 100 GB')
+    t, meta, _, _ = make(5, C, H, H, seed=3, post='rms', pre='layer')
+    v = {k: u.cuda() for k, u in t.items() if u is not None and k not in 'xb'}
+    meta.pop('rows_per_sample')
+    big = lambda seed: torch.empty(rows, C, device='cuda', dtype=H).normal_(generator=torch.Generator('cuda').manual_seed(seed))  # noqa: E731
+    x, b, dh, dy = (big(k) for k in range(4))
+    last = slice(rows - 5, rows)
+    back = {k: u for k, u in v.items() if k != 'pre_b'}
+    h, y, st = ops.resnorm_fwd(x, b, **v, **meta, rows_per_sample=rows)
+    dx, db, _, _ = ops.resnorm_bwd(dh, dy, h, b, st, **back, **meta, rows_per_sample=rows)
+    h1, y1, st1 = ops.resnorm_fwd(x[last], b[last], **v, **meta, rows_per_sample=5)
+    dx1, db1, _, _ = ops.resnorm_bwd(dh[last], dy[last], h1, b[last], st1, **back, **meta, rows_per_sample=5)
+    for p, q in ((h, h1), (y, y1), (st, st1), (dx, dx1), (db, db1)):
+        assert torch.equal(p[last], q)
+    del x, b, dh, dy, h, y, dx, db, st
+    torch.cuda.empty_cache()
+
+
+def captured_training(C=48):
+    torch.manual_seed(3)
+    leaves = [torch.randn(2, 9, C, device='cuda').requires_grad_(), torch.randn(2, 9, C, device='cuda').requires_grad_(),
+              (torch.rand(C, device='cuda') + 0.5).requires_grad_(), (torch.rand(C, device='cuda') + 0.5).requires_grad_()]
+    dh, dy = torch.randn(2, 9, C, device='cuda'), torch.randn(2, 9, C, device='cuda')
+
+    def forward():
+        from semseg_amd.resnorm import gated_residual_norm
+        return gated_residual_norm(leaves[0], leaves[1], post='rms', post_weight=leaves[2], pre='rms', pre_weight=leaves[3])
+    return leaves, (dh, dy), forward
+
+
+@pytest.mark.parametrize('accumulate', [False, True])
+def test_captured_autograd_backward(accumulate):
+    """two captured training passes of the same leaves replay the eager bits, with eager passes in between"""
+    leaves, dout, forward = captured_training()
+
+    def step():
+        if not accumulate:
+            return list(torch.autograd.grad(forward(), leaves, dout))
+        torch.autograd.backward(forward(), dout)
+        return [p.grad for p in leaves]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        for p in leaves:
+            p.grad = None
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, out))
+    for k in range(4):
+        with torch.no_grad():
+            leaves[0].mul_(1.5), leaves[1].add_(0.25)
+        for p in leaves:
+            p.grad = None
+        eager = torch.autograd.grad(forward(), leaves, dout)
+        for g, out in graphs:
+            for v in out:
+                v.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(out, eager)), k
+
+
+def test_a_captured_backward_is_refused_while_an_eager_graph_of_its_leaves_lives():
+    leaves, dout, forward = captured_training()
+    alive = forward()                                          # made on the default stream, never run backward
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match='eager graph of the same leaves'):
+            torch.autograd.grad(forward(), leaves, dout)
+        with pytest.raises(RuntimeError, match='eager graph of the same leaves'):
+            torch.autograd.backward(forward(), dout)
+        out = forward()                                        # the forward alone is taken
+    assert all(p.grad is None for p in leaves)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(out, alive))
