@@ -573,3 +573,29 @@ def test_a_captured_backward_is_refused_while_an_eager_graph_of_its_leaves_lives
     g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(out, alive))
+
+
+def test_checkpointing_and_saved_tensor_hooks():
+    """recomputed and offloaded activations give the gradients of the plain graph; a second backward of a freed graph is refused"""
+    from torch.utils.checkpoint import checkpoint
+    leaves, dout, forward = captured_training()
+    want = torch.autograd.grad(forward(), leaves, dout)
+    for reentrant in (False, True):
+        got = torch.autograd.grad(checkpoint(lambda *a: forward(), *leaves, use_reentrant=False), leaves, dout) if not reentrant else None
+        if reentrant:
+            torch.autograd.backward(checkpoint(lambda *a: forward(), *leaves, use_reentrant=True), dout)
+            got = [p.grad for p in leaves]
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    with torch.autograd.graph.save_on_cpu():
+        out = forward()
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(out, leaves, dout), want))
+    with pytest.raises(RuntimeError, match='second time|already been freed'):
+        torch.autograd.grad(out, leaves, dout)
+    out = forward()
+    assert out[0].requires_grad and not out[0].is_leaf and out[1].grad_fn is out[0].grad_fn or out[1].grad_fn.name() == out[0].grad_fn.name()
+    with torch.no_grad():
+        assert not forward()[0].requires_grad
+    seen = []
+    out[0].register_hook(lambda g: seen.append(tuple(g.shape)))
+    torch.autograd.grad(out, leaves[:1], dout)                 # one input alone
+    assert seen == [(2, 9, 48)]
