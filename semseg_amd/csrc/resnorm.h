@@ -6,50 +6,64 @@
 // Row starts need no alignment beyond the element's (odd widths, odd row strides): global memory takes the access as one.
 struct __attribute__((packed, aligned(2))) Bf8u { bf16x8 v; };
 struct __attribute__((packed, aligned(4))) Fl8u { floatx4 a, b; };
-template <typename T> struct Chunk;
-template <> struct Chunk<bf16> {
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+struct __attribute__((packed, aligned(2))) Bf6u { unsigned a, b, c; };
+struct __attribute__((packed, aligned(4))) Fl6u { floatx4 a; floatx2 b; };
+template <typename T, int E> struct Chunk;
+template <> struct Chunk<bf16, 8> {
     bf16x8 v;
     __device__ __forceinline__ void load(const bf16* p) { v = ((const Bf8u*)p)->v; }
     __device__ __forceinline__ float get(int e) const { return (float)v[e]; }
     __device__ __forceinline__ void set(int e, float f) { v[e] = (bf16)f; }
     __device__ __forceinline__ void store(bf16* p) const { ((Bf8u*)p)->v = v; }
 };
-template <> struct Chunk<float> {
+template <> struct Chunk<bf16, 6> {
+    unsigned v[3];
+    __device__ __forceinline__ void load(const bf16* p) { const Bf6u t = *(const Bf6u*)p; v[0] = t.a; v[1] = t.b; v[2] = t.c; }
+    __device__ __forceinline__ float get(int e) const { return __uint_as_float(e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16); }
+    __device__ __forceinline__ void set(int e, float f) { bf16x2 t = __builtin_bit_cast(bf16x2, v[e >> 1]); t[e & 1] = (bf16)f; v[e >> 1] = __builtin_bit_cast(unsigned, t); }
+    __device__ __forceinline__ void store(bf16* p) const { *(Bf6u*)p = Bf6u{v[0], v[1], v[2]}; }
+};
+template <> struct Chunk<float, 6> {
+    floatx4 a;
+    floatx2 b;
+    __device__ __forceinline__ void load(const float* p) { a = ((const Fl6u*)p)->a; b = ((const Fl6u*)p)->b; }
+    __device__ __forceinline__ float get(int e) const { return e < 4 ? a[e & 3] : b[e & 1]; }
+    __device__ __forceinline__ void set(int e, float f) { if (e < 4) a[e & 3] = f; else b[e & 1] = f; }
+    __device__ __forceinline__ void store(float* p) const { ((Fl6u*)p)->a = a; ((Fl6u*)p)->b = b; }
+};
+template <> struct Chunk<float, 8> {
     floatx4 a, b;
     __device__ __forceinline__ void load(const float* p) { a = ((const Fl8u*)p)->a; b = ((const Fl8u*)p)->b; }
     __device__ __forceinline__ float get(int e) const { return e < 4 ? a[e & 3] : b[e & 3]; }
     __device__ __forceinline__ void set(int e, float f) { if (e < 4) a[e & 3] = f; else b[e & 3] = f; }
     __device__ __forceinline__ void store(float* p) const { ((Fl8u*)p)->a = a; ((Fl8u*)p)->b = b; }
 };
-// The eight channels of a lane: [cb, cb + 8), of which e in [lo, hi) count as its own.  At the end of a row whose width is no multiple of
-// eight the last chunk is moved back to end with the row, and a lane past the row's end reads that chunk too and owns nothing: every load
-// is a whole chunk inside the row, without a branch.  (A load under a branch may not have been issued, so a wait for an older one has to
-// wait for everything, and the next row's loads are not in flight any more: ConvNeXt stage 3 backward 101 us against 75.)  What two lanes
+template <typename T> struct Chunk<T, 1> {
+    T v;
+    __device__ __forceinline__ void load(const T* p) { v = *p; }
+    __device__ __forceinline__ float get(int) const { return to_f(v); }
+    __device__ __forceinline__ void set(int, float f) { v = from_f<T>(f); }
+    __device__ __forceinline__ void store(T* p) const { *p = v; }
+};
+// The E channels of a lane: eight, six where that leaves fewer lanes idle, one in rows of less than eight, so that C >= E always.  They are
+// [cb, cb + E), of which those from lo on count as its own.  At the end of a row whose width is no multiple of E the last chunk is moved
+// back to end with the row, and a lane past the row's end reads that chunk too and owns nothing (lo = E): every load is a whole chunk
+// inside the row, WITHOUT A BRANCH, not even one that the whole launch takes alike: behind a branch the compiler cannot count the loads
+// in flight, a wait for one row's loads becomes a wait for all, and the next row's are not on their way any more (bf16, LN + LN +
+// gate, 24 M elements, backward: C = 500 73 -> 65 us, 4096 100 -> 82; forward 500 50 -> 44, 4096 44 -> 40).  What two lanes
 // hold of the same channel is the same to the last bit, so the moved chunk is stored whole as well; only sums count a channel once.
-struct Cols { int cb, lo, hi; };
-__device__ __forceinline__ Cols cols_of(int c, int C) {
+struct Cols { int cb, lo; };
+template <int E> __device__ __forceinline__ Cols cols_of(int c, int C) {
     const int n = C - c;
     Cols r;
-    r.cb = n >= 8 ? c : C >= 8 ? C - 8 : 0;
-    r.lo = n >= 8 ? 0 : n <= 0 ? 8 : C >= 8 ? 8 - n : 0;
-    r.hi = C >= 8 ? 8 : C;
+    r.cb = n >= E ? c : C - E;
+    r.lo = n >= E ? 0 : n <= 0 ? E : E - n;
     return r;
 }
 // compared where it is used: sixteen lane masks kept over a loop do not fit the scalar registers
-__device__ __forceinline__ Cols here(Cols k) { asm volatile("" : "+v"(k.lo), "+v"(k.hi)); return k; }
-// a row of less than eight channels is loaded one by one (every lane of the launch alike)
-template <typename T> __device__ __forceinline__ void load_chunk(Chunk<T>& t, const T* p, int C) {
-    if (C >= 8) t.load(p);
-    else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) t.set(e, to_f(p[e < C ? e : C - 1]));
-    }
-}
-template <typename T> __device__ __forceinline__ void store_chunk(const Chunk<T>& t, T* p, int C) {
-    if (C >= 8) { t.store(p); return; }
-#pragma unroll
-    for (int e = 0; e < 7; ++e) if (e < C) p[e] = from_f<T>(t.get(e));
-}
+__device__ __forceinline__ Cols here(Cols k) { asm volatile("" : "+v"(k.lo)); return k; }
 
 // Address of a lane's element: a row that the whole wave agrees on (64 bits, scalar registers) and the lane's offset from it (32 bits): one
 // vector register a tensor instead of two for every pointer.  The host keeps 64 row strides below 2^32 bytes.
@@ -107,24 +121,38 @@ template <int WAVES> __device__ __forceinline__ void row_stats(double s, double 
 __device__ __forceinline__ float sigmoid_f(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 
 // ---------------------------------------------------------------- the vectors (weights, biases, scale) in LDS
-// One row of `chunks` chunks per vector, the two halves of a chunk apart: lanes read 16 bytes each, 16 bytes apart.
-__device__ __forceinline__ void stage_vec(float* sh, const float* p, float otherwise, int C, int chunks, int threads) {
-    for (int i = threadIdx.x; i < chunks * 8; i += threads) {
-        const int c = cols_of(i & ~7, C).cb + (i & 7);
-        sh[((i >> 2) & 1) * chunks * 4 + (i >> 3) * 4 + (i & 3)] = c >= C ? 0.f : p ? p[c] : otherwise;
+// One row of `chunks` chunks per vector, the first four and the other channels of a chunk apart: lanes read 16 bytes each, 16 bytes apart,
+// then 16 or 8.
+template <int E> __device__ __forceinline__ void put_chunk(float* sh, const float (&v)[E], int chunk, int chunks) {
+    if constexpr (E == 1) sh[chunk] = v[0];
+    else {
+        *(floatx4*)(sh + chunk * 4) = floatx4{v[0], v[1], v[2], v[3]};
+        if constexpr (E == 8) *(floatx4*)(sh + chunks * 4 + chunk * 4) = floatx4{v[4], v[5], v[6], v[7]};
+        else *(floatx2*)(sh + chunks * 4 + chunk * 2) = floatx2{v[4], v[5]};
     }
 }
-// the same for a thread that owns its columns (C > 8)
-__device__ __forceinline__ void load_vec(float (&v)[8], const float* p, float otherwise, const Cols& k) {
-    Chunk<float> t;
+// a lane's chunk of a vector, or the value that stands for one that is not given
+template <int E> __device__ __forceinline__ void load_vec(float (&v)[E], const float* p, float otherwise, const Cols& k) {
+    Chunk<float, E> t;
     if (p) t.load(p + k.cb);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = p ? t.get(e) : otherwise;
+    for (int e = 0; e < E; ++e) v[e] = p ? t.get(e) : otherwise;
 }
-__device__ __forceinline__ void vec_chunk(float (&v)[8], const float* sh, int chunk, int chunks) {
-    const floatx4 a = *(const floatx4*)(sh + chunk * 4), b = *(const floatx4*)(sh + chunks * 4 + chunk * 4);
+template <int E> __device__ __forceinline__ void vec_chunk(float (&v)[E], const float* sh, int chunk, int chunks) {
+    if constexpr (E == 1) v[0] = sh[chunk];
+    else {
+        const floatx4 a = *(const floatx4*)(sh + chunk * 4);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+        for (int e = 0; e < 4; ++e) v[e] = a[e];
+        if constexpr (E == 8) {
+            const floatx4 b = *(const floatx4*)(sh + chunks * 4 + chunk * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 + e] = b[e];
+        } else {
+            const floatx2 b = *(const floatx2*)(sh + chunks * 4 + chunk * 2);
+            v[4] = b[0]; v[5] = b[1];
+        }
+    }
 }
 
 // ---------------------------------------------------------------- C ABI: what both entries check
