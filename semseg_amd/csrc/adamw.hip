@@ -136,7 +136,8 @@ __device__ __forceinline__ float step_coef(const AdamArgs& a, const AdamDyn* __r
     return clip_coef(norm, a.max_norm, a.grad_scale);
 }
 
-// One workgroup: joins the partial sums in a fixed order, counts the step, and leaves what the update reads.
+// One workgroup: joins the partial sums in a fixed order, counts the step, and leaves what the update reads.  4.7 us, all latency, which is
+// why small models join the sums in the update instead.
 struct AdamSchedule { double lr[SS_ADAMW_GROUPS], wd[SS_ADAMW_GROUPS]; };
 __global__ __launch_bounds__(256) void adamw_prepare_kernel(const double* __restrict__ partial, int64_t count, double max_norm, double grad_scale,
         double beta1, double beta2, int64_t t_host, int64_t* __restrict__ t_dev, AdamSchedule sched, const double* __restrict__ lr_dev, int groups,
@@ -179,6 +180,8 @@ __device__ __forceinline__ void adam_moments(float g, float& m, float& v, const 
     v = vb + vg;
 }
 
+// 28 bytes an element in f32 (16 of them moments): 24 M elements 125 us = 5.4 TB/s, as fast as a copy.  Two vectors of each of the four
+// streams in flight a thread; a chunk of at most 8192 elements, so that every workgroup is resident at once up to 16 M.
 template <typename TP, typename TG>
 __global__ __launch_bounds__(256) void adamw32_kernel(AdamPtrs2 ptrs, const AdamChunk* __restrict__ plan, int first_tensor, float* __restrict__ m,
         float* __restrict__ v, AdamArgs a, const AdamDyn* __restrict__ dyn) {
@@ -250,6 +253,9 @@ __device__ __forceinline__ float decode_m(unsigned word, int e) {           // s
     return c * fabsf(c);
 }
 
+// 16 bytes an element and 1/16 in f32: 81 M elements 246 us = 5.3 TB/s; 3.3 M 18 us, 4.4 M of bf16 24 us.  447 vector instructions for four
+// elements a lane, 34 of them at a quarter of the rate, take about as long as the bytes: more loads in flight (a resident grid with the
+// next run on its way) cost more in registers than they gave (246 -> 270 us).
 template <typename TP, typename TG>
 __global__ __launch_bounds__(256) void adamw8_kernel(AdamPtrs2 ptrs, const AdamChunk* __restrict__ plan, int first_tensor, unsigned* __restrict__ mc,
         unsigned* __restrict__ vc, float* __restrict__ qm, float* __restrict__ qv, AdamArgs a, const AdamDyn* __restrict__ dyn) {
@@ -303,7 +309,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamPtrs2 ptrs, const AdamC
     }
 }
 
-// the moments that 8-bit codes stand for
+// the moments that 8-bit codes stand for: 2 bytes in, 8 out; 81 M elements 156 us = 5.2 TB/s
 __global__ __launch_bounds__(256) void adamw8_values_kernel(const unsigned* __restrict__ mc, const unsigned* __restrict__ vc, const float* __restrict__ qm,
         const float* __restrict__ qv, float* __restrict__ m, float* __restrict__ v, int64_t words) {
     const int64_t stride = (int64_t)gridDim.x * 256;

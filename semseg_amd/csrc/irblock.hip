@@ -144,7 +144,7 @@ __global__ __launch_bounds__(256, 4) void ir_block_kernel(IrArgs a, int ntiles, 
                     const floatx4 w0 = *(const floatx4*)(wb + (ky * K + kx) * a.hidp), w1 = *(const floatx4*)(wb + (ky * K + kx) * a.hidp + 4);
                     const floatx2 wv[4] = {floatx2{w0[0], w0[1]}, floatx2{w0[2], w0[3]}, floatx2{w1[0], w1[1]}, floatx2{w1[2], w1[3]}};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {                 // a bf16 pair widens with one shift and one mask; the products are packed fp32 fmas
+                    for (int e = 0; e < 4; ++e) {                 // a bf16 pair widens with one shift and one mask; the products are fp32 fmas
                         const floatx2 hv = {__uint_as_float(h.w[e] << 16), __uint_as_float(h.w[e] & 0xffff0000u)};
                         u[e] = __builtin_elementwise_fma(hv, wv[e], u[e]);
                     }

@@ -7,7 +7,7 @@
 //   A  expand:    h1[halo pixel][slice] = x . W1[slice]^T + b1 on the matrix cores (v_mfma_f32_32x32x16_bf16, weights as the A operand
 //                 so a lane is a pixel), zero outside the image (the depthwise conv pads h1), bf16 into LDS -- the rounding point of
 //                 the three-launch form;
-//   B  depthwise: 8 channels x 1 pixel per item from 16-byte LDS gathers, taps in registers, GELU in packed fp32, bf16 into a second
+//   B  depthwise: 8 channels x 1 pixel per item from 16-byte LDS gathers, taps in registers, GELU on pairs, bf16 into a second
 //                 LDS image (the second rounding point);
 //   C  project:   out[pixel][C] += a2[pixel][slice] . W2[:, slice]^T, accumulators stay in registers across the slices;
 // then bias, DropPath scale and residual in fp32 and one rounding, as the GEMM epilogue does.  The x fragments of the tile's halo
@@ -26,7 +26,7 @@ struct MixArgs {
 
 // GELU(u) = u Phi(u) for a pair, Abramowitz-Stegun 7.1.26 as gelu_parts (common.h): Phi(u) = 1/2 + sign(u) (1/2 - hc),
 // hc = 1/2 erfc(|u| / sqrt 2) = poly(t) exp(-u^2 / 2), t = 1 / (1 + p |u| / sqrt 2)  =>  GELU(u) = u / 2 + |u| (1/2 - hc).
-// Packed fp32 where the ISA has it (v_pk_mul / v_pk_fma); |u| rides as the abs modifier of two plain fmas.
+// Written on pairs; the build keeps packed fp32 instructions off, so each is two plain ones, and |u| rides as the abs modifier of two fmas.
 __device__ __forceinline__ floatx2 gelu2(floatx2 u, floatx2& hc_out, floatx2& ez_out) {
     floatx2 t, ez;
     t[0] = __builtin_amdgcn_rcpf(fmaf(fabsf(u[0]), 0.3275911f * 0.70710678118654752f, 1.f));

@@ -1,8 +1,8 @@
 // Host side of the calls whose cost is the host's: the autograd node of the gated residual norm and the address lists of the optimizer.
 //
 // A training call on a few thousand rows is 30 us of GPU work; as a Python autograd.Function it is 160 us of host work, half of it in the
-// backward, which autograd runs on another thread with the interpreter's lock in between; here it is 78.  Here the node is C++: checks, allocations and
-// launches without the interpreter.  The kernels are those of the C ABI; their addresses are handed over by init(), from the library that
+// backward, which autograd runs on another thread with the interpreter's lock in between.  Here the node is C++: checks, allocations and
+// launches without the interpreter, 78 us.  The kernels are those of the C ABI; their addresses are handed over by init(), from the library that
 // the Python side has loaded, so there is one library whatever its path.
 #include <torch/extension.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>

@@ -66,6 +66,7 @@ __host__ __device__ constexpr int bwd_waves(int width, int waves, bool narrow, b
     return narrow ? (!post && gate == 0 ? 4 : 3) : post ? 2 : 3;
 }
 
+// Measured (sizes as at the forward): 176 us = 4.7 TB/s, 63 us = 4.8, 142 us = 5.2; the join behind it 4 to 5 us.
 template <typename TX, typename TB, int E, int WAVES, bool POST, int GATE>
 __global__ __launch_bounds__(WAVES > 1 ? WAVES * 64 : 256, bwd_waves(E, WAVES, sizeof(TX) == 2, POST, GATE)) void resnorm_bwd_kernel(ResnormBwdArgs a) {
     constexpr int THREADS = WAVES > 1 ? WAVES * 64 : 256;

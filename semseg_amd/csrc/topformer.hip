@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256) void inject_fuse_kernel(const T* __restrict__ 
 // out = local * up(ga) + up(ge) + sum_i up(extra_i): the injection of the finest stage and the SimpleHead's UniRes + Sum over the other
 // stages in one pass over the finest map (the sum used to be three read-modify-write passes over it); fp32 until the one rounding.
 // A workgroup walks output rows: the vertical taps of every source are per-row constants, a thread owns 8 channels of a pixel, the four
-// taps enter with their products l_y * l_x as packed fp32 fmas (bf16 pairs widen with one shift and one mask), and the flat index is
+// taps enter with their products l_y * l_x as fp32 fmas (bf16 pairs widen with one shift and one mask), and the flat index is
 // decomposed by multiply-shift (the 64-bit divisions of a flat grid cost more than the arithmetic).
 struct UpSrc { const void* p; int64_t ld; int h, w; float sh, sw; };       // sh, sw: source / destination size
 struct UpSrc3 { UpSrc s[3]; int n; };
