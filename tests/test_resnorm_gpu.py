@@ -599,3 +599,33 @@ def test_checkpointing_and_saved_tensor_hooks():
     out[0].register_hook(lambda g: seen.append(tuple(g.shape)))
     torch.autograd.grad(out, leaves[:1], dout)                 # one input alone
     assert seen == [(2, 9, 48)]
+
+
+@pytest.mark.parametrize('types', TYPES)
+@pytest.mark.parametrize('C', [2, 3, 6, 7, 9, 11, 12, 18, 23, 90, 96, 200, 330, 384, 385, 600, 767, 768, 1023, 1100, 1535, 1536, 2047, 2100, 2500])
+def test_chunks_of_one_six_and_eight_channels(C, types):
+    """both norms, gates and DropPath where the chunk's width or the waves of a row change, one workgroup and many"""
+    for rows, samples, gate in ((7, 1, 'row'), (390, 3, 'sample')):
+        t, meta, dh, dy = make(rows, C, *types, seed=C, samples=samples, post='layer', pre='rms', gate=gate, act='sigmoid', keep=True, alpha=0.75)
+        run_and_check(t, meta, dh, dy)
+
+
+@pytest.mark.parametrize('C', [5, 96, 700, 1300])
+def test_views_of_every_chunk_width(C):
+    """rows at odd offsets and strides: the bits of the dense call, and nothing written next to the rows"""
+    from semseg_amd import ops
+    for types in TYPES:
+        t, meta, dh, dy = make(33, C, *types, seed=1, samples=3, post='rms', pre='layer', gate='sample')
+        d = {k: None if v is None else v.cuda() for k, v in t.items()}
+
+        def odd(v):
+            wide = torch.zeros(v.shape[0], C + 5, device='cuda', dtype=v.dtype)
+            wide[:, 3:3 + C] = v.cuda()
+            return wide[:, 3:3 + C]
+        o = {**d, 'x': odd(t['x']), 'b': odd(t['b'])}
+        dense, view = ops.resnorm_fwd(**d, **meta), ops.resnorm_fwd(**o, **meta)
+        assert all(torch.equal(p, q) for p, q in zip(dense, view))
+        back = {k: v for k, v in d.items() if k not in ('x', 'b', 'pre_b')}
+        one = ops.resnorm_bwd(dh.cuda(), dy.cuda(), dense[0], d['b'], dense[2], **back, **meta)
+        two = ops.resnorm_bwd(odd(dh), odd(dy), dense[0], o['b'], dense[2], **back, **meta)
+        assert all(torch.equal(p, q) for p, q in zip(one[:3], two[:3])) and all(torch.equal(one[3][k], two[3][k]) for k in one[3])
