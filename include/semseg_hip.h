@@ -620,7 +620,8 @@ int ss_adamw_clip_step(int p_dtype, int g_dtype, int bits, int count, void* cons
 int ss_adamw8_values(const void* m, const void* v, const float* m_scale, const float* v_scale, float* m_out, float* v_out, int64_t runs,
                      hipStream_t stream);
 
-/* ---- gradient delivery: dst[i][0..numel[i]) += src[i] for `count` fp32 tensors in one launch per 40 tensors.  Source i is
+/* ---- gradient delivery: dst[i][0..numel[i]) += src[i] for `count` fp32 tensors in one launch per 40 tensors.  A destination may repeat
+ * or overlap an earlier one: it is then added to by a later launch, in list order.  Source i is
  * numel[i] / cols[i] rows of cols[i] contiguous floats, src_ld[i] apart (cols[i] == numel[i]: contiguous); dst[i] is contiguous.
  * src, src_ld, cols, dst and numel are HOST arrays.  Replaces autograd's per-parameter AccumulateGrad adds (what DDP's reducer
  * does when it copies gradients into its buckets, train.py:306) when the gradients live in one flat buffer (engine.FlatParams). */

@@ -93,15 +93,21 @@ __global__ __launch_bounds__(256) void multi_add_kernel(MultiAddTable t) {
 extern "C" int ss_multi_add_f32(int count, const float* const* src, const int64_t* src_ld, const int64_t* cols, float* const* dst,
                                 const int64_t* numel, hipStream_t stream) {
     SS_CHECK(count >= 0 && (count == 0 || (src && src_ld && cols && dst && numel)), "ss_multi_add_f32: bad arguments");
-    for (int i0 = 0; i0 < count; i0 += SS_MULTI_MAX) {
+    for (int k = 0; k < count; ++k)
+        SS_CHECK(src[k] && dst[k] && numel[k] > 0 && cols[k] > 0 && cols[k] < (1LL << 31) && numel[k] % cols[k] == 0 &&
+                 (cols[k] == numel[k] || src_ld[k] >= cols[k]), "ss_multi_add_f32: bad tensor %d (numel %lld cols %lld ld %lld)", k,
+                 (long long)numel[k], (long long)cols[k], (long long)src_ld[k]);
+    for (int k = 0; k < count;) {
         MultiAddTable t;
-        t.count = count - i0 < SS_MULTI_MAX ? count - i0 : SS_MULTI_MAX;
+        t.count = 0;
         int64_t blocks = 0;
-        for (int i = 0; i < t.count; ++i) {
-            const int k = i0 + i;
-            SS_CHECK(src[k] && dst[k] && numel[k] > 0 && cols[k] > 0 && cols[k] < (1LL << 31) && numel[k] % cols[k] == 0 &&
-                     (cols[k] == numel[k] || src_ld[k] >= cols[k]), "ss_multi_add_f32: bad tensor %d (numel %lld cols %lld ld %lld)", k,
-                     (long long)numel[k], (long long)cols[k], (long long)src_ld[k]);
+        for (; k < count && t.count < SS_MULTI_MAX; ++k) {
+            // workgroups add with a plain load and store: what an entry of this launch already writes (a parameter in two roles of one
+            // node) waits for the next launch, which the stream puts behind this one
+            bool taken = false;
+            for (int i = 0; i < t.count; ++i) taken |= dst[k] < t.dst[i] + t.n[i] && t.dst[i] < dst[k] + numel[k];
+            if (taken) break;
+            const int i = t.count++;
             t.src[i] = src[k]; t.dst[i] = dst[k]; t.n[i] = numel[k]; t.ld[i] = src_ld[k]; t.cols[i] = (int)cols[k];
             t.first_block[i] = (int)blocks;
             blocks += cdiv(numel[k], SS_MULTI_PER_BLOCK);

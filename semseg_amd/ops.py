@@ -1707,7 +1707,8 @@ def multi_add_layout(t):
 
 
 def multi_add(srcs, dsts):
-    """dsts[i] += srcs[i] for lists of fp32 device tensors (dsts contiguous, srcs as multi_add_layout allows), one launch per 40."""
+    """dsts[i] += srcs[i] for lists of fp32 device tensors (dsts contiguous, srcs as multi_add_layout allows), one launch per 40;
+    a destination that repeats or overlaps an earlier one is added to behind it."""
     import ctypes
     n = len(srcs)
     if n == 0:
