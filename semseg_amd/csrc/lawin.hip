@@ -381,7 +381,9 @@ __global__ __launch_bounds__(256) void lawin_attn_bwd_kernel(const T* __restrict
         store_d<T, D, VEC>(dtheta + row * lddt + hd * D, acc);
     }
     T* drow = dpg + (wi * 64 + lane) * (2 * (int64_t)inter) + hd * D;
-    // pass B reads this lane's phi and g rows again from LDS: held in registers across pass A they take the D = 64 kernel past 512 (spills)
+    // pass B reads this lane's phi and g rows again from LDS: held in registers across pass A they take the D = 64 kernel in f32 past 512, and
+    // the compiler (ROCm 7.2.0) then brings back only three of the four registers of one group: two had gone to scratch memory, two to
+    // accumulation registers, and gk[2] stayed whatever its place held (dphi wrong in every lane).  With this the kernel has no scratch.
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int d = 0; d < D; ++d) { pk[d] = ph[lane * D + d]; gk[d] = gg[lane * D + d]; }
