@@ -195,6 +195,12 @@ Forward forward_with_graph(const Tensor& x, const Tensor& b, const Tensor& gate,
 typedef std::optional<Tensor> Maybe;
 Tensor or_none(const Maybe& t) { return t ? *t : Tensor(); }
 
+// The kernels write new tensors behind the dispatcher's back: what follows a computation by watching it would see nothing of this one.
+void refuse_watchers(const std::vector<Maybe>& inputs) {
+    for (const Maybe& t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(0).defined(), "gated_residual_norm: no forward-mode derivatives are built");
+}
+
 py::object gated_residual_norm(const Tensor& x, const Tensor& branch, int post, const Maybe& post_w_, const Maybe& post_b_, const Maybe& gate_, int act,
                                const Maybe& scale_, const Maybe& keep_, double alpha, int pre, const Maybe& pre_w_, const Maybe& pre_b_, double eps,
                                int64_t samples, const std::vector<Maybe>& sinks) {
@@ -202,6 +208,7 @@ py::object gated_residual_norm(const Tensor& x, const Tensor& branch, int post, 
                  pre_w = or_none(pre_w_), pre_b = or_none(pre_b_);
     typedef py::value_error Value;
     typedef py::type_error Type;
+    refuse_watchers({x, branch, gate_, post_w_, post_b_, pre_w_, pre_b_, scale_, keep_});
     if (x.dim() < 2 || !x.sizes().equals(branch.sizes()))
         fail<Value>("x " + str(x.sizes()) + " and branch " + str(branch.sizes()) + " must be alike, [..., C]");
     Cfg c{0, 0, x.size(-1), 0, post, pre, act, alpha, eps, {}};
@@ -282,5 +289,6 @@ void init(uint64_t fwd, uint64_t ws, uint64_t bwd, uint64_t add, uint64_t err) {
 PYBIND11_MODULE(_native, m) {
     m.def("init", &init);
     m.def("gated_residual_norm", &gated_residual_norm);
+    m.def("refuse_watchers", &refuse_watchers);
     m.def("addresses", &addresses);
 }

@@ -77,7 +77,7 @@ def gated_residual_norm(x: Tensor, branch: Tensor, *, post='none', post_weight=N
     x, branch: [..., C], alike; float32 / float32, bfloat16 / bfloat16 or a float32 stream around a bfloat16 branch.  post, pre: 'none', 'layer'
     (weight, optionally bias) or 'rms' (weight).  gate (branch's type): per sample [samples, C] or per element, shaped like x; gate_act:
     'none' or 'sigmoid'.  scale, weights, biases: float32 [C].  keep: float32 [samples].  A sample is an index of x's first dimension (a 2-D
-    x is one sample) unless ``samples`` says into how many equal runs of rows x divides.  Differentiable in everything but keep."""
+    x is one sample) unless ``samples`` says into how many equal runs of rows x divides.  Differentiable in everything but keep, by backward only: forward-mode derivatives are refused."""
     vectors = (pre_weight, pre_bias, post_weight, post_bias, scale)
     if _lib.TRACE is None and not any(hasattr(v, '_ss_grad_ready') for v in vectors):
         if post not in ops._NORM or pre not in ops._NORM or gate_act not in ops._GATE_ACT:
@@ -89,6 +89,7 @@ def gated_residual_norm(x: Tensor, branch: Tensor, *, post='none', post_weight=N
                                                  ops._NORM[pre], pre_weight, pre_bias, eps, samples or 0,
                                                  sinks if any(s is not None for s in sinks) else [])
     # parameters whose gradients an engine.GradReducer waits for (its callbacks are Python), and traced calls: the same node in Python
+    _lib.native().refuse_watchers([x, branch, gate, keep, *vectors])
     shape = x.shape
     if len(shape) < 2 or branch.shape != shape:
         raise ValueError(f'gated_residual_norm: x {tuple(shape)} and branch {tuple(branch.shape)} must be alike, [..., C]')
