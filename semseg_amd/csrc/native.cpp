@@ -7,11 +7,14 @@
 #include <torch/extension.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <string>
 #include <vector>
@@ -195,8 +198,12 @@ Forward forward_with_graph(const Tensor& x, const Tensor& b, const Tensor& gate,
 typedef std::optional<Tensor> Maybe;
 Tensor or_none(const Maybe& t) { return t ? *t : Tensor(); }
 
+typedef c10::impl::TorchDispatchModeTLS Modes;
 // The kernels write new tensors behind the dispatcher's back: what follows a computation by watching it would see nothing of this one.
 void refuse_watchers(const std::vector<Maybe>& inputs) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() && !Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY) &&
+                                !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch),
+                                "gated_residual_norm: tracing would record outputs that nothing computes; it is not built");
     for (const Maybe& t : inputs)
         TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(0).defined(), "gated_residual_norm: no forward-mode derivatives are built");
 }

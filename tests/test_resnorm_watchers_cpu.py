@@ -41,3 +41,38 @@ def test_jvp_is_refused(node):
     t = inputs()
     with pytest.raises(NotImplementedError, match='forward-mode'):
         torch.func.jvp(lambda v: gated_residual_norm(v, t['branch'])[0], (t['x'],), (t['x'],))
+
+
+def joined(v):
+    return gated_residual_norm(v, v + 1)[0]
+
+
+def test_jit_trace_is_refused(node):
+    with pytest.raises(NotImplementedError, match='tracing'):
+        torch.jit.trace(joined, (torch.rand(2, 3, 8),), check_trace=False)
+
+
+@pytest.mark.parametrize('kw', [{}, {'tracing_mode': 'fake'}, {'tracing_mode': 'symbolic'}, {'pre_dispatch': True}, {'tracing_mode': 'symbolic', 'pre_dispatch': True}])
+def test_make_fx_is_refused(node, kw):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    with pytest.raises(NotImplementedError, match='tracing'):
+        make_fx(joined, **kw)(torch.rand(2, 3, 8))
+    with pytest.raises(NotImplementedError, match='tracing'):
+        make_fx(torch.no_grad()(joined), **kw)(torch.rand(2, 3, 8))
+
+
+def test_nothing_is_refused_once_tracing_ended(node):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for _ in range(2):
+        with pytest.raises(NotImplementedError, match='tracing'):
+            make_fx(joined)(torch.rand(2, 3, 8))
+        with pytest.raises(RuntimeError, match='HIP device'):
+            joined(torch.rand(2, 3, 8))
+
+
+def test_export_is_refused(node):
+    class Join(torch.nn.Module):
+        def forward(self, v):
+            return joined(v)
+    with pytest.raises(Exception):                            # whatever the exporter wraps it in
+        torch.export.export(Join(), (torch.rand(2, 3, 8),), strict=False)
