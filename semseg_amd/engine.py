@@ -471,36 +471,74 @@ class AdamW:
                    'params': sorted(idx for idx, j, _, _, _ in self._slots() if self.group_of[j] == i)} for i, (s, w) in enumerate(self.groups)]
         return {'state': dict(sorted(state.items())), 'param_groups': groups, 'lr': self.lr, 'weight_decay': self.wd}
 
-    def load_state_dict(self, sd):
-        group = sd['param_groups'][0]
-        if group.get('amsgrad') or group.get('maximize'):
-            raise ValueError('AdamW.load_state_dict: amsgrad and maximize are not built')
-        if int(group.get('state_bits', 32)) != self.state_bits:
-            raise ValueError(f'AdamW.load_state_dict: moments in {group.get("state_bits", 32)} bits, this optimizer holds {self.state_bits}')
-        if 'lr' in sd:
-            self.lr, self.wd = float(sd['lr']), float(sd['weight_decay'])
-        elif len(sd['param_groups']) == 1:                     # a torch.optim.AdamW checkpoint
-            self.lr, self.wd = float(group['lr']), float(group['weight_decay'])
-        self.betas, self.eps, self.seed = tuple(group['betas']), float(group['eps']), int(group.get('seed', self.seed))
-        steps = set()
+    def load_state_dict(self, sd, order=None):
+        """Takes what ``state_dict()`` gave, or a ``torch.optim.AdamW`` checkpoint.  torch numbers parameters through its groups: with more
+        than one group say in ``order`` which parameter each number stands for (the parameters, group after group, as they were given to
+        it); the groups' rates and decays have to be those of ``per_param``.  A checkpoint that is refused leaves everything as it was."""
+        def refuse(why):
+            raise ValueError('AdamW.load_state_dict: ' + why)
+        groups, own, n = sd['param_groups'], 'lr' in sd, len(self.params)
+        for g in groups:
+            if g.get('amsgrad') or g.get('maximize'):
+                refuse('amsgrad and maximize are not built')
+            if int(g.get('state_bits', 32)) != self.state_bits:
+                refuse(f'moments in {g.get("state_bits", 32)} bits, this optimizer holds {self.state_bits}')
+        betas, eps = tuple(float(b) for b in groups[0]['betas']), float(groups[0]['eps'])
+        if any((tuple(float(b) for b in g['betas']), float(g['eps'])) != (betas, eps) for g in groups):
+            refuse('groups with different betas or eps; one of each is kept')
+        if not (len(betas) == 2 and all(0.0 <= b < 1.0 for b in betas) and eps >= 0.0):
+            refuse(f'betas {betas}, eps {eps}')
+        if order is not None:
+            order = list(order)
+            place = {id(p): i for i, p in enumerate(order)}
+            if len(order) != n or set(place) != {id(p) for p in self.params}:
+                refuse('order must name each parameter once')
+            index_of = [place[id(p)] for p in self.params]
+        elif not own and len(groups) > 1:
+            refuse(f'{len(groups)} groups: say in order which parameter each number stands for')
+        else:
+            index_of = [idx for idx, *_ in self._slots()]
+        of = {int(i): g for g in groups for i in g['params']}
+        if sorted(of) != list(range(n)) or any(int(i) not in of for i in sd['state']):
+            refuse(f'parameters {sorted(of)} and state {sorted(int(i) for i in sd["state"])}, this optimizer has {n}')
+        # rates and decays: one of each, times what per_param says
+        if own or len(groups) == 1:
+            lr, wd = (float((sd if own else groups[0])[k]) for k in ('lr', 'weight_decay'))
+            saved = [(g['lr_scale'], float(g['weight_decay'])) if own else None for g in (of[i] for i in index_of)]
+        else:
+            lr = next((float(of[i]['lr']) / self.groups[k][0] for i, k in zip(index_of, self.group_of) if self.groups[k][0] > 0.0), 0.0)
+            wd = next((float(of[i]['weight_decay']) for i, k in zip(index_of, self.group_of) if self.groups[k][1] is None), self.wd)
+            saved = [(float(of[i]['lr']) / lr if lr > 0.0 else self.groups[k][0], float(of[i]['weight_decay'])) for i, k in zip(index_of, self.group_of)]
+        if not (lr >= 0.0 and wd >= 0.0):
+            refuse(f'lr {lr}, weight_decay {wd}')
+        for i, k, was in zip(index_of, self.group_of, saved):
+            scale, decay = self.groups[k][0], wd if self.groups[k][1] is None else self.groups[k][1]
+            if was is not None and (abs(was[0] - scale) > 1e-9 * scale or abs(was[1] - decay) > 1e-9 * decay):
+                refuse(f'parameter {i} was trained at {was[0]:g} times the rate with decay {was[1]:g}, here at {scale:g} with {decay:g}')
+        steps, copies = set(), []
+        for idx, (_, j, p, run, runs) in zip(index_of, self._slots()):
+            st = sd['state'].get(idx, sd['state'].get(str(idx)))
+            o, k = run * ops.ADAMW_RUN, p.numel()
+            pairs = [(self.exp_avg[o:o + k], 'exp_avg', p.shape), (self.exp_avg_sq[o:o + k], 'exp_avg_sq', p.shape)]
+            if self.state_bits == 8:
+                pairs += [(self.exp_avg_scale[run:run + runs], 'exp_avg_scale', (runs,)), (self.exp_avg_sq_scale[run:run + runs], 'exp_avg_sq_scale', (runs,))]
+            for dst, name, shape in pairs:
+                if st is None:                                 # a parameter that has not been stepped yet
+                    copies.append((dst, None))
+                    continue
+                src = st.get(name)
+                if src is None or tuple(src.shape) != tuple(shape) or src.is_floating_point() != dst.is_floating_point():
+                    refuse(f'state {idx} has {name} {None if src is None else (tuple(src.shape), src.dtype)}, expected {tuple(shape)} {dst.dtype}')
+                copies.append((dst, src.detach().reshape(-1)))
+            if st is not None:
+                steps.add(int(st['step']))
+        if len(steps) > 1 or any(t < 0 for t in steps):
+            refuse(f'parameters at different steps {sorted(steps)}; one step count is kept')
+        # nothing is refused from here on
+        self.lr, self.wd, self.betas, self.eps, self.seed = lr, wd, betas, eps, int(groups[0].get('seed', self.seed))
         with torch.no_grad():
-            for idx, _, p, run, runs in self._slots():
-                st = sd['state'].get(idx, sd['state'].get(str(idx)))
-                o, n = run * ops.ADAMW_RUN, p.numel()
-                pairs = [(self.exp_avg[o:o + n], 'exp_avg', p.shape), (self.exp_avg_sq[o:o + n], 'exp_avg_sq', p.shape)]
-                if self.state_bits == 8:
-                    pairs += [(self.exp_avg_scale[run:run + runs], 'exp_avg_scale', (runs,)), (self.exp_avg_sq_scale[run:run + runs], 'exp_avg_sq_scale', (runs,))]
-                for dst, name, shape in pairs:
-                    if st is None:                             # a parameter that has not been stepped yet
-                        dst.zero_()
-                        continue
-                    if tuple(st[name].shape) != tuple(shape):
-                        raise ValueError(f'AdamW.load_state_dict: state {idx} has {name} of shape {tuple(st[name].shape)}, expected {tuple(shape)}')
-                    dst.copy_(st[name].reshape(-1))
-                if st is not None:
-                    steps.add(int(st['step']))
-        if len(steps) > 1:
-            raise ValueError(f'AdamW.load_state_dict: parameters at different steps {sorted(steps)}; one step count is kept')
+            for dst, src in copies:
+                dst.zero_() if src is None else dst.copy_(src)
         self.t = steps.pop() if steps else 0
         if self._lr_dev is not None:
             self.push_lr()
