@@ -10,13 +10,13 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
-#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 using at::Tensor;
@@ -101,21 +101,34 @@ void deliver(const std::vector<Tensor>& sinks, const variable_list& params, Tens
 }
 
 // A leaf's gradient is handed over on the stream on which the oldest living graph used the leaf.  In a capture that must not be the default
-// stream: the capture cannot take its work in, and the process ends over it.  So such a backward is refused before it gets there.
+// stream: the capture cannot take its work in, and the process ends over it.  The same holds for any other node that was made there.  So such
+// a backward is refused before it gets there, for everything that this node's gradients reach, through views and other nodes too.  (Nodes
+// that come before this one in the backward have had their turn by then.)
 void refuse_default_stream_leaves(const torch::autograd::Node& node) {
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
     const auto* info = torch::autograd::get_current_graph_task_exec_info();
-    for (const auto& edge : node.next_edges()) {
-        auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
-        if (!leaf) continue;
-        if (info && !info->empty()) {                                        // autograd.grad: only what is asked for; it goes to the leaf's stream too
-            const auto it = info->find(leaf);
-            if (it == info->end() || !it->second.should_execute()) continue;
+    std::vector<const torch::autograd::Node*> open{&node};
+    std::unordered_set<const torch::autograd::Node*> seen;
+    while (!open.empty()) {
+        const torch::autograd::Node* at = open.back();
+        open.pop_back();
+        for (const auto& edge : at->next_edges()) {
+            auto* next = edge.function.get();
+            if (!next || !seen.insert(next).second) continue;
+            if (info && !info->empty()) {                                    // autograd.grad: only what is asked for; it goes to the leaf's stream too
+                const auto it = info->find(next);
+                if (it == info->end() || !it->second.should_execute()) continue;
+            }
+            const auto s = next->stream();
+            TORCH_CHECK(!s || s->id() != 0, "gated_residual_norm: backward captured while an eager graph of the same leaves, made on the default stream, is alive; "
+                        "drop its outputs first, or run the eager passes on a side stream");
+            open.push_back(next);
         }
-        const auto s = leaf->stream();
-        TORCH_CHECK(!s || s->id() != 0, "gated_residual_norm: backward captured while an eager graph of the same leaves, made on the default stream, is alive; "
-                    "drop its outputs first, or run the eager passes on a side stream");
     }
+}
+// for a node whose backward is Python, while it runs
+void refuse_captured_leaves() {
+    if (const auto node = torch::autograd::get_current_node()) refuse_default_stream_leaves(*node);
 }
 
 // The node itself, with members of its own: torch::autograd::Function keeps what it saves in a dictionary of boxed values and dispatches every
@@ -297,5 +310,6 @@ PYBIND11_MODULE(_native, m) {
     m.def("init", &init);
     m.def("gated_residual_norm", &gated_residual_norm);
     m.def("refuse_watchers", &refuse_watchers);
+    m.def("refuse_captured_leaves", &refuse_captured_leaves);
     m.def("addresses", &addresses);
 }

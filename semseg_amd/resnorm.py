@@ -55,6 +55,7 @@ class _ResnormFn(GradAwareFunction):
             raise RuntimeError('gated_residual_norm: no gradients of gradients (create_graph=True) are built')
         if dh is None and dy is None:
             return (None,) * 10
+        _lib.native().refuse_captured_leaves()
         rows, n, C, mode, post, pre, act, alpha, _ = ctx.cfg
         h, b, gate, keep, stats, *vectors = ctx.saved_tensors
         _, _, post_w, post_b, scale = vectors
