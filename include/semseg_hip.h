@@ -585,7 +585,7 @@ int ss_resnorm_bwd(int x_dtype, int b_dtype, const void* dh, int64_t lddh, const
 /* ---- AdamW (Loshchilov & Hutter 2019) over many tensors in one launch, with the global gradient norm and clipping; moments in 32 bits or
  * in 8.  The reference trains with AdaBound only (train.py:53-58); this is the optimizer that the published recipes of its encoders use.
  *   g' = coef g;  m = b1 m + (1-b1) g';  v = b2 v + (1-b2) g'^2;  p = (1 - lr wd) p - lr / (1-b1^t) m / (sqrt(v) / sqrt(1-b2^t) + eps)
- *   coef = grad_scale min(1, max_norm / (norm + 1e-6)),  norm = grad_scale |all gradients| (squares summed in double)
+ *   coef = grad_scale min(1, max_norm / (norm + 1e-6)),  norm = |grad_scale| |all gradients| (squares summed in double)
  * Tensors are given as HOST arrays of device addresses (params, grads; contiguous, aligned to their element) and a PLAN in device memory
  * that holds no address: one record of four 64-bit words per chunk of a tensor,
  *   { first element in the tensor;  elements | first run << 32;  tensor | group << 32;  0 },

@@ -2,7 +2,7 @@
 //
 // Mathematics (Loshchilov & Hutter, ICLR 2019), per element with g' = coef g:
 //   m = b1 m + (1-b1) g';  v = b2 v + (1-b2) g'^2;  p = (1 - lr wd) p - lr / (1-b1^t) m / (sqrt(v) / sqrt(1-b2^t) + eps)
-//   coef = grad_scale min(1, max_norm / (norm + 1e-6)),  norm = grad_scale |g| over ALL tensors
+//   coef = grad_scale min(1, max_norm / (norm + 1e-6)),  norm = |grad_scale g| over ALL tensors
 // The squares are summed in double: the product of two floats is exact there, so the norm, and with it coef, does not depend on the
 // order of the sum in any bit that survives the rounding to float.
 //
@@ -131,7 +131,7 @@ __device__ __forceinline__ float step_coef(const AdamArgs& a, const AdamDyn* __r
     if (dyn) return dyn->coef;
     if (!a.partial) return a.dyn.coef;
     __shared__ double sh[4];
-    const double norm = sqrt(join_sums(a.partial, a.sums, sh)) * a.grad_scale;
+    const double norm = sqrt(join_sums(a.partial, a.sums, sh)) * fabs(a.grad_scale);
     if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = (float)norm;
     return clip_coef(norm, a.max_norm, a.grad_scale);
 }
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256) void adamw_prepare_kernel(const double* __rest
         dyn->decay[threadIdx.x] = (float)(1.0 - lr * sched.wd[threadIdx.x]);
     }
     if (threadIdx.x == 0) {
-        const double norm = sqrt(sum) * grad_scale;
+        const double norm = sqrt(sum) * fabs(grad_scale);
         const int skip = skip_nonfinite && !(norm < __builtin_huge_val());  // infinite or NaN
         if (t_dev && !skip) *t_dev = t_s;
         if (norm_out) *norm_out = (float)norm;
