@@ -83,6 +83,20 @@ Forward launch_forward(const Tensor& x, const Tensor& b, const Tensor& gate, con
     return r;
 }
 
+// autograd.grad and backward(inputs=...): gradients of some tensors only, or to be handed to the caller
+bool some_gradients_only() {
+    const auto* info = torch::autograd::get_current_graph_task_exec_info();
+    return info && !info->empty();
+}
+// in such a pass, a parameter's gradient goes where autograd takes it: to the caller, or nowhere
+bool left_to_autograd(const Tensor& p) {
+    if (!some_gradients_only()) return false;
+    const auto* info = torch::autograd::get_current_graph_task_exec_info();
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(p);
+    const auto it = info->find(accumulator.get());
+    return it == info->end() || !it->second.needed_ || it->second.captures_;
+}
+
 // What runtime.deliver_grads does: gradients whose parameter still has its slot as .grad are added there, all in one launch, and autograd is
 // handed nothing for them.
 void deliver(const std::vector<Tensor>& sinks, const variable_list& params, Tensor* grads, void* stream) {
@@ -93,7 +107,7 @@ void deliver(const std::vector<Tensor>& sinks, const variable_list& params, Tens
     for (int i = 0; i < 5; ++i) {
         const Tensor &g = grads[i], &p = params[i];
         if (!g.defined() || !sinks[i].defined() || !p.requires_grad() || !p.grad().defined() || p.grad().const_data_ptr() != sinks[i].const_data_ptr() ||
-            sinks[i].numel() != g.numel()) continue;
+            sinks[i].numel() != g.numel() || left_to_autograd(p)) continue;
         src[k] = g.const_data_ptr<float>(); dst[k] = sinks[i].mutable_data_ptr<float>(); n[k] = g.numel(); at[k++] = i;
     }
     if (k) check(multi_add(k, src, n, n, dst, n, stream));
@@ -311,5 +325,7 @@ PYBIND11_MODULE(_native, m) {
     m.def("gated_residual_norm", &gated_residual_norm);
     m.def("refuse_watchers", &refuse_watchers);
     m.def("refuse_captured_leaves", &refuse_captured_leaves);
+    m.def("some_gradients_only", &some_gradients_only);
+    m.def("left_to_autograd", &left_to_autograd);
     m.def("addresses", &addresses);
 }

@@ -3,7 +3,7 @@ import threading
 import warnings
 import torch
 
-from . import ops
+from . import _lib, ops
 
 _FORCED = None
 
@@ -89,12 +89,16 @@ def deliver_grads(params, grads):
     """What a backward node returns for its parameters.  A parameter that engine.FlatParams has given a slot in the flat
     gradient buffer (``_ss_grad_sink``) receives its gradient there -- ALL such gradients of the node in one ``ss_multi_add_f32``
     launch, with accumulate semantics like autograd's -- and autograd is handed None for it; its ``_ss_grad_ready`` callback
-    (the bucketed all-reduce of engine.GradReducer) fires once the launch is queued.  Everything else goes back to autograd."""
+    (the bucketed all-reduce of engine.GradReducer) fires once the launch is queued.  Everything else goes back to autograd, and so do the
+    gradients that ``torch.autograd.grad`` hands to its caller and those that ``backward(inputs=...)`` leaves out."""
     out, srcs, dsts, ready = [], [], [], []
+    native = _lib.native()
+    some = native.some_gradients_only()
     for p, g in zip(params, grads):
         sink = getattr(p, '_ss_grad_sink', None)
         if g is None or sink is None or g.dtype != torch.float32 or g.numel() != sink.numel() or g.numel() == 0 \
-                or ops.multi_add_layout(g) is None or p.grad is None or p.grad.data_ptr() != sink.data_ptr():
+                or ops.multi_add_layout(g) is None or p.grad is None or p.grad.data_ptr() != sink.data_ptr() \
+                or (some and native.left_to_autograd(p)):
             out.append(g)
             continue
         srcs.append(g), dsts.append(sink), out.append(None)

@@ -82,3 +82,29 @@ def run_parts(x, b, dh, dy, values, roles, names):
 
 def sum_of_parts(parts):
     return sum(p.abs() for p in parts)
+
+
+@pytest.mark.parametrize('python', [False, True])
+def test_flat_parameters_under_autograd_grad_and_some_inputs(python):
+    """the gradients of a plain module, handed to the caller or put into the slots that are asked for, and nothing anywhere else"""
+    from semseg_amd.engine import FlatParams
+    from semseg_amd.resnorm import GatedResidualNorm
+    torch.manual_seed(5)
+    plain, flat = (GatedResidualNorm(40, post='layer', pre='rms', layer_scale=0.5).cuda() for _ in range(2))
+    buffer = FlatParams(flat)
+    if python:
+        for p in flat.parameters():
+            p._ss_grad_ready = lambda q: None
+    x, b = (torch.randn(3, 5, 40, device='cuda', requires_grad=True) for _ in range(2))
+
+    def loss(m):
+        h, y = m(x, b)
+        return h.square().sum() + (y * x.detach()).sum()
+    for pick in (lambda m: [x, *m.parameters()], lambda m: [b], lambda m: [m.scale, m.pre_weight]):
+        want, got = torch.autograd.grad(loss(plain), pick(plain)), torch.autograd.grad(loss(flat), pick(flat))
+        assert all(torch.equal(p, q) for p, q in zip(want, got)) and not buffer.grad.any()
+    loss(plain).backward(inputs=[plain.scale, plain.post_bias])
+    loss(flat).backward(inputs=[flat.scale, flat.post_bias])
+    assert torch.equal(flat.scale.grad, plain.scale.grad) and torch.equal(flat.post_bias.grad, plain.post_bias.grad)
+    assert not flat.pre_weight.grad.any() and not flat.post_weight.grad.any() and x.grad is None
+    assert flat.scale.grad.data_ptr() == flat.scale._ss_grad_sink.data_ptr()
