@@ -30,8 +30,15 @@ def native_command():
             '-L' + os.path.join(root, 'lib'), '-ltorch', '-ltorch_cpu', '-ltorch_hip', '-lc10', '-lc10_hip', '-ltorch_python']
 
 
-def _newer(src, dst, deps):
+def _stamp(src):
+    return os.path.join(OBJ, os.path.basename(src) + '.command')
+
+
+def _newer(src, dst, deps, command):
+    """whether dst has to be made: it is missing, older than a source, or was made by another command (other flags, another torch)"""
     if not os.path.exists(dst):
+        return True
+    if not os.path.exists(_stamp(src)) or open(_stamp(src)).read() != ' '.join(command):
         return True
     t = os.path.getmtime(dst)
     return any(os.path.getmtime(p) > t for p in [src] + deps)
@@ -45,20 +52,24 @@ def build(force=False, verbose=True):
     jobs = []
     for s in srcs:
         src, obj = os.path.join(CSRC, s), os.path.join(OBJ, s[:-4] + '.o')
-        if force or _newer(src, obj, hdrs):
-            jobs.append((src, obj))
-
-    native = os.path.join(CSRC, 'native.cpp')
+        cmd = [hipcc] + FLAGS + ['-c', src, '-o', obj]
+        if force or _newer(src, obj, hdrs, cmd):
+            jobs.append((src, cmd))
 
     def cc(job):
-        src, obj = job
-        cmd = native_command() if src == native else [hipcc] + FLAGS + ['-c', src, '-o', obj]
+        src, cmd = job
+        if os.path.exists(_stamp(src)):
+            os.remove(_stamp(src))                             # a command that fails or is cut off leaves none
         r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode == 0:
+            with open(_stamp(src), 'w') as f:
+                f.write(' '.join(cmd))
         return src, r.returncode, r.stderr
 
     device_jobs = bool(jobs)
-    if force or _newer(native, NATIVE, []):
-        jobs.append((native, NATIVE))
+    native, cmd = os.path.join(CSRC, 'native.cpp'), native_command()
+    if force or _newer(native, NATIVE, [], cmd):
+        jobs.append((native, cmd))
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
         for src, rc, err in ex.map(cc, jobs):
             if verbose:
@@ -66,7 +77,7 @@ def build(force=False, verbose=True):
             if rc != 0:
                 raise RuntimeError(f'compiling {src} failed:\n{err}')
     objs = [os.path.join(OBJ, s[:-4] + '.o') for s in srcs]
-    if force or device_jobs or not os.path.exists(LIB):
+    if force or device_jobs or not os.path.exists(LIB) or any(os.path.getmtime(o) > os.path.getmtime(LIB) for o in objs):
         r = subprocess.run([hipcc, '--offload-arch=gfx950', '-shared', '-fPIC', '-o', LIB] + objs, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError('link failed:\n' + r.stderr)
