@@ -310,6 +310,22 @@ py::tuple addresses(const std::vector<Tensor>& params, const std::vector<int64_t
     return py::make_tuple(gt < 0 ? 0 : gt, py::bytes((const char*)pa.data(), pa.size() * 8), py::bytes((const char*)ga.data(), ga.size() * 8));
 }
 
+// Parameters that are to lie, with their gradients, at `offsets` of two flat float buffers; the handles are kept, what they hold is looked at
+// by each call (turning a list of 186 parameters into handles is 8 us)
+struct FlatSlots {
+    std::vector<Tensor> params;
+    std::vector<int64_t> offsets;
+    // -> the first that lies elsewhere, or -1
+    int64_t first_stray(uint64_t data, uint64_t grad) const {
+        for (size_t i = 0; i < params.size(); ++i) {
+            const Tensor &p = params[i], &g = p.grad();
+            if (p.numel() == 0) continue;
+            if ((uint64_t)p.const_data_ptr() != data + 4 * offsets[i] || !g.defined() || (uint64_t)g.const_data_ptr() != grad + 4 * offsets[i]) return i;
+        }
+        return -1;
+    }
+};
+
 void init(uint64_t fwd, uint64_t ws, uint64_t bwd, uint64_t add, uint64_t err) {
     resnorm_fwd = (fwd_fn)fwd;
     resnorm_ws = (ws_fn)ws;
@@ -328,4 +344,10 @@ PYBIND11_MODULE(_native, m) {
     m.def("some_gradients_only", &some_gradients_only);
     m.def("left_to_autograd", &left_to_autograd);
     m.def("addresses", &addresses);
+    py::class_<FlatSlots>(m, "FlatSlots")
+        .def(py::init([](std::vector<Tensor> params, std::vector<int64_t> offsets) {
+            TORCH_CHECK(params.size() == offsets.size(), "FlatSlots: an offset for each parameter");
+            return FlatSlots{std::move(params), std::move(offsets)};
+        }))
+        .def("first_stray", &FlatSlots::first_stray);
 }

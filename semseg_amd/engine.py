@@ -327,6 +327,7 @@ class AdamW:
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=None, state_bits=32, seed=0, per_param=None,
                  skip_nonfinite=False, capturable=False):
         self.flat = params if isinstance(params, FlatParams) else None
+        self._slots_of_flat = None
         self.params = list(self.flat.params if self.flat is not None else params)
         if not self.params:
             raise ValueError('AdamW: no parameters')
@@ -405,6 +406,13 @@ class AdamW:
         few hundred tensors cost more than their step)"""
         if self.flat is not None:
             f = self.flat
+            if self._slots_of_flat is None:
+                self._slots_of_flat = native().FlatSlots(self.params, f.offsets)
+            stray = self._slots_of_flat.first_stray(f.data.data_ptr(), f.grad.data_ptr())
+            if stray >= 0:
+                raise RuntimeError(f'AdamW: parameter {stray} of the flat buffers, {tuple(self.params[stray].shape)}, or its .grad lies elsewhere, and the buffers '
+                                   'hold old values for it: clear gradients with FlatParams.zero_grad() (or zero_grad(set_to_none=False)), '
+                                   'change parameters in place')
             return 0, f.data.data_ptr().to_bytes(8, 'little'), f.grad.data_ptr().to_bytes(8, 'little')
         return native().addresses(self.params, self.numels, ops._DT[self.dtype], self.device.index)
 
