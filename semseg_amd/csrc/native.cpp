@@ -88,13 +88,19 @@ bool some_gradients_only() {
     const auto* info = torch::autograd::get_current_graph_task_exec_info();
     return info && !info->empty();
 }
-// in such a pass, a parameter's gradient goes where autograd takes it: to the caller, or nowhere
+// Whether a parameter's gradient is autograd's to place, not the node's: in such a pass it goes to the caller, or nowhere; and where the
+// parameter's accumulator belongs to another stream than the one at work, only autograd's own hand-over makes the caller's stream wait
+// (in a capture the node's launch is part of the graph, and a hand-over to a stream outside would break it).
 bool left_to_autograd(const Tensor& p) {
-    if (!some_gradients_only()) return false;
-    const auto* info = torch::autograd::get_current_graph_task_exec_info();
     const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(p);
-    const auto it = info->find(accumulator.get());
-    return it == info->end() || !it->second.needed_ || it->second.captures_;
+    if (some_gradients_only()) {
+        const auto* info = torch::autograd::get_current_graph_task_exec_info();
+        const auto it = info->find(accumulator.get());
+        if (it == info->end() || !it->second.needed_ || it->second.captures_) return true;
+    }
+    if (!accumulator || !p.is_cuda() || c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) return false;
+    const auto s = accumulator->stream();
+    return s && *s != c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(p.device().index()).unwrap();
 }
 
 // What runtime.deliver_grads does: gradients whose parameter still has its slot as .grad are added there, all in one launch, and autograd is
@@ -341,7 +347,6 @@ PYBIND11_MODULE(_native, m) {
     m.def("gated_residual_norm", &gated_residual_norm);
     m.def("refuse_watchers", &refuse_watchers);
     m.def("refuse_captured_leaves", &refuse_captured_leaves);
-    m.def("some_gradients_only", &some_gradients_only);
     m.def("left_to_autograd", &left_to_autograd);
     m.def("addresses", &addresses);
     py::class_<FlatSlots>(m, "FlatSlots")

@@ -90,15 +90,15 @@ def deliver_grads(params, grads):
     gradient buffer (``_ss_grad_sink``) receives its gradient there -- ALL such gradients of the node in one ``ss_multi_add_f32``
     launch, with accumulate semantics like autograd's -- and autograd is handed None for it; its ``_ss_grad_ready`` callback
     (the bucketed all-reduce of engine.GradReducer) fires once the launch is queued.  Everything else goes back to autograd, and so do the
-    gradients that ``torch.autograd.grad`` hands to its caller and those that ``backward(inputs=...)`` leaves out."""
+    gradients that ``torch.autograd.grad`` hands to its caller, those that ``backward(inputs=...)`` leaves out, and those of a parameter whose
+    accumulator was made on another stream (autograd makes the streams wait for one another)."""
     out, srcs, dsts, ready = [], [], [], []
     native = _lib.native()
-    some = native.some_gradients_only()
     for p, g in zip(params, grads):
         sink = getattr(p, '_ss_grad_sink', None)
         if g is None or sink is None or g.dtype != torch.float32 or g.numel() != sink.numel() or g.numel() == 0 \
                 or ops.multi_add_layout(g) is None or p.grad is None or p.grad.data_ptr() != sink.data_ptr() \
-                or (some and native.left_to_autograd(p)):
+                or native.left_to_autograd(p):
             out.append(g)
             continue
         srcs.append(g), dsts.append(sink), out.append(None)

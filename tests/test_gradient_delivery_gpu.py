@@ -108,3 +108,37 @@ def test_flat_parameters_under_autograd_grad_and_some_inputs(python):
     assert torch.equal(flat.scale.grad, plain.scale.grad) and torch.equal(flat.post_bias.grad, plain.post_bias.grad)
     assert not flat.pre_weight.grad.any() and not flat.post_weight.grad.any() and x.grad is None
     assert flat.scale.grad.data_ptr() == flat.scale._ss_grad_sink.data_ptr()
+
+
+@pytest.mark.parametrize('python', [False, True])
+def test_a_forward_on_another_stream_than_the_leaves(python):
+    """leaves whose accumulators belong to the caller's stream, a graph made on a side stream: the caller sees its gradients without waiting itself"""
+    from semseg_amd.engine import FlatParams
+    from semseg_amd.resnorm import GatedResidualNorm
+    torch.manual_seed(6)
+    m = GatedResidualNorm(40, post='layer', pre='rms', layer_scale=0.5).cuda()
+    flat = FlatParams(m)
+    if python:
+        for p in m.parameters():
+            p._ss_grad_ready = lambda q: None
+    x, b = torch.randn(3, 5, 40, device='cuda'), torch.randn(3, 5, 40, device='cuda')
+
+    def loss():
+        h, y = m(x, b)
+        return h.square().sum() + (y * x).sum()
+    loss().backward()
+    torch.cuda.synchronize()
+    want = flat.grad.clone()
+    flat.zero_grad()
+    alive = [p * 1.0 for p in m.parameters()]                  # accumulators on the caller's stream
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for k in range(3):
+        with torch.cuda.stream(side):
+            value = loss()
+            torch.cuda._sleep(20_000_000)                      # some 10 ms: the backward's kernels wait behind it
+        value.backward()
+        got = flat.grad.clone()                                # on the caller's stream, without a word to the side stream
+        torch.cuda.synchronize()
+        assert torch.allclose(got, (k + 1) * want, rtol=2.0 ** -23, atol=0), k      # the third sum and product are rounded once each
+    assert all(p.grad.data_ptr() == p._ss_grad_sink.data_ptr() for p in m.parameters()) and alive
