@@ -405,15 +405,15 @@ class AdamW:
         """-> code of the gradients' type, HOST arrays of the parameters' and gradients' addresses (checked in C++: in Python the checks of a
         few hundred tensors cost more than their step)"""
         if self.flat is not None:
-            f = self.flat
+            data, grad = self.flat.data.data_ptr(), self.flat.grad.data_ptr()
             if self._slots_of_flat is None:
-                self._slots_of_flat = native().FlatSlots(self.params, f.offsets)
-            stray = self._slots_of_flat.first_stray(f.data.data_ptr(), f.grad.data_ptr())
+                self._slots_of_flat = native().FlatSlots(self.params, self.flat.offsets)
+            stray = self._slots_of_flat.first_stray(data, grad)
             if stray >= 0:
                 raise RuntimeError(f'AdamW: parameter {stray} of the flat buffers, {tuple(self.params[stray].shape)}, or its .grad lies elsewhere, and the buffers '
                                    'hold old values for it: clear gradients with FlatParams.zero_grad() (or zero_grad(set_to_none=False)), '
                                    'change parameters in place')
-            return 0, f.data.data_ptr().to_bytes(8, 'little'), f.grad.data_ptr().to_bytes(8, 'little')
+            return 0, data.to_bytes(8, 'little'), grad.to_bytes(8, 'little')
         return native().addresses(self.params, self.numels, ops._DT[self.dtype], self.device.index)
 
     def step(self, grad_scale=1.0):
