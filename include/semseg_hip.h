@@ -562,7 +562,8 @@ int ss_adabound_step(float* p, const float* g, float* m, float* v, int64_t n, do
                      float step_size, float lower, float upper, float weight_decay, float grad_scale, hipStream_t stream);
 
 /* ---- the residual update between two blocks with a norm on either side of it (LayerScale / gated / sandwich-norm residual blocks; the
- * reference has the plain form x + drop_path(gamma * f(norm(x))), modules/convnext.py:38-51, modules/segformer.py:94-98):
+ * reference has x + drop_path(branch) and the next norm, modules/segformer.py:94-98, and x + drop_path(gamma * branch) without one,
+ * modules/convnext.py:38-51):
  *   n = post(b);  h = alpha x + keep[s] scale[c] act(gate) n;  y = pre(h)        r < 2^30 rows of sample s = r / rows_per_sample, C <= 4096 channels
  * post, pre: 0 none, 1 LayerNorm (weight, bias may be NULL), 2 RMSNorm (weight); gate_mode: 0 none, 1 one row of C per sample, 2 one per row;
  * act: 0 identity, 1 sigmoid.  x and h have x_dtype, b, gate and y b_dtype: f32 / f32, bf16 / bf16 or f32 / bf16.  x, b, gate (and the

@@ -4,7 +4,8 @@
 // Column sums (the vectors' gradients, a per-sample gate's) stay in registers over all rows of a workgroup: eight channels a lane, up to 48
 // accumulators, which is what limits a lane to one chunk; the vectors themselves are read from LDS.  A workgroup walks UNITS: rows of
 // one sample, so a per-sample gate's gradient is flushed once a unit.  Partial sums of the workgroups are joined by a second, small
-// launch in a fixed order; nothing is atomic.
+// launch in a fixed order; nothing is atomic.  An accumulator adds one term for each row that its lane takes, in 32 bits: at most
+// rows / (workgroups x rows at once) of them, 4096 for 2^20 rows of 4096 channels, then 48 + 32 in the join (up to 1536 workgroups).
 #pragma once
 #include "resnorm.h"
 
@@ -58,8 +59,9 @@ template <int WAVES, typename D = float, int E> __device__ __forceinline__ void 
 template <typename TX, typename TB, int E, bool GATE> struct BwdRow { Chunk<TX, E> dh, h; Chunk<TB, E> dy, b, g[1]; float keep; floatx4 st; };
 
 // Waves a SIMD, which bounds the registers (512 / waves); the grid is what is resident then: a second, partial round of workgroups would
-// run at a fraction of the waves (MiT stage 1: 1024 workgroups 203 us, 768 169 us).  Rows that several waves share in eights, bf16: one less,
-// for no spills and fewer partial sums (LN + LN + gate, 24 M elements, C = 1024 81 -> 68 us; in sixes it would cost, 640 73 -> 81).
+// run at a fraction of the waves.  bf16 without a post norm or gate: four, which is between (join included, 16 x 65536 x 64 174 us, three 167;
+// 65536 x 320 50, three 53; 65536 x 384 58, three 57).  Rows that several waves share in eights, bf16: one less, for fewer partial sums
+// (LN + LN + gate, 24 M elements, C = 1024 81 -> 68 us; in sixes it would cost, 640 73 -> 81).
 __host__ __device__ constexpr int bwd_waves(int width, int waves, bool narrow, bool post, int gate) {
     if (waves > 4) return 2;
     if (narrow && waves > 1 && width == 8) return post ? 2 : 3;

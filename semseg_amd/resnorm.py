@@ -2,8 +2,11 @@
 
     n = post(branch);   h = alpha * x + keep[s] * scale * act(gate) * n;   y = pre(h)
 
-The reference writes the plain form of it, ``x + drop_path(gamma * branch)`` followed by the next block's LayerNorm
-(modules/convnext.py:38-51, modules/segformer.py:94-98).  ``post`` normalises what a block hands over before it joins the stream (sandwich
+The reference's MiT blocks write the plain form of it, ``x + drop_path(branch)`` followed by the next norm (modules/segformer.py:94-98); its
+ConvNeXt blocks end in ``x + drop_path(gamma * branch)`` and no norm, the next block's comes behind its depthwise convolution
+(modules/convnext.py:38-51): ``pre='none'``.  This package's own MiT and ConvNeXt have residual, LayerScale and DropPath in the epilogue of the product
+that makes the branch; the operator is for blocks put together by hand, where the branch comes from anything else.
+``post`` normalises what a block hands over before it joins the stream (sandwich
 norm), ``pre`` is the norm that the next block starts with, ``scale`` is LayerScale, ``gate`` modulates per sample (conditioned
 blocks) or per element (gated blocks), ``keep`` is DropPath's multiplier (``runtime.drop_path_keep``) and ``alpha`` the weight of the
 residual (DeepNorm).  Activations are token matrices, fp32 or bf16, or an fp32 stream around bf16 blocks; statistics, sums and all
