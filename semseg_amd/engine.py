@@ -481,8 +481,9 @@ class AdamW:
 
     def load_state_dict(self, sd, order=None):
         """Takes what ``state_dict()`` gave, or a ``torch.optim.AdamW`` checkpoint.  torch numbers parameters through its groups: with more
-        than one group say in ``order`` which parameter each number stands for (the parameters, group after group, as they were given to
-        it); the groups' rates and decays have to be those of ``per_param``.  A checkpoint that is refused leaves everything as it was."""
+        than one group, or with parameters that this optimizer does not hold (frozen ones), say in ``order`` which parameter each number
+        stands for: the parameters as they were given to it, group after group.  The rates and decays of several groups have to be those of
+        ``per_param``.  A checkpoint that is refused leaves everything as it was."""
         def refuse(why):
             raise ValueError('AdamW.load_state_dict: ' + why)
         groups, own, n = sd['param_groups'], 'lr' in sd, len(self.params)
@@ -499,16 +500,16 @@ class AdamW:
         if order is not None:
             order = list(order)
             place = {id(p): i for i, p in enumerate(order)}
-            if len(order) != n or set(place) != {id(p) for p in self.params}:
+            if len(place) != len(order) or not all(id(p) in place for p in self.params):
                 refuse('order must name each parameter once')
-            index_of = [place[id(p)] for p in self.params]
+            index_of, n = [place[id(p)] for p in self.params], len(order)
         elif not own and len(groups) > 1:
             refuse(f'{len(groups)} groups: say in order which parameter each number stands for')
         else:
             index_of = [idx for idx, *_ in self._slots()]
         of = {int(i): g for g in groups for i in g['params']}
         if sorted(of) != list(range(n)) or any(int(i) not in of for i in sd['state']):
-            refuse(f'parameters {sorted(of)} and state {sorted(int(i) for i in sd["state"])}, this optimizer has {n}')
+            refuse(f'parameters {sorted(of)} and state {sorted(int(i) for i in sd["state"])}, {n} parameters expected (order names others)')
         # rates and decays: one of each, times what per_param says
         if own or len(groups) == 1:
             lr, wd = (float((sd if own else groups[0])[k]) for k in ('lr', 'weight_decay'))
@@ -535,7 +536,7 @@ class AdamW:
                     copies.append((dst, None))
                     continue
                 src = st.get(name)
-                if src is None or tuple(src.shape) != tuple(shape) or src.is_floating_point() != dst.is_floating_point():
+                if src is None or tuple(src.shape) != tuple(shape) or (src.dtype != dst.dtype if self.state_bits == 8 else not src.is_floating_point()):
                     refuse(f'state {idx} has {name} {None if src is None else (tuple(src.shape), src.dtype)}, expected {tuple(shape)} {dst.dtype}')
                 copies.append((dst, src.detach().reshape(-1)))
             if st is not None:

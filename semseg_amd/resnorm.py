@@ -81,8 +81,8 @@ def gated_residual_norm(x: Tensor, branch: Tensor, *, post='none', post_weight=N
     x, branch: [..., C], alike; float32 / float32, bfloat16 / bfloat16 or a float32 stream around a bfloat16 branch.  post, pre: 'none', 'layer'
     (weight, optionally bias) or 'rms' (weight).  gate (branch's type): per sample [samples, C] or per element, shaped like x; gate_act:
     'none' or 'sigmoid'.  scale, weights, biases: float32 [C].  keep: float32 [samples].  A sample is an index of x's first dimension (a 2-D
-    x is one sample) unless ``samples`` says into how many equal runs of rows x divides.  Differentiable in everything but keep, by backward only: forward-mode derivatives are
-    refused, and so is tracing (torch.jit.trace, make_fx, export)."""
+    x is one sample) unless ``samples`` says into how many equal runs of rows x divides.  Differentiable in everything but keep,
+    by backward only: forward-mode derivatives are refused, and so is tracing (torch.jit.trace, make_fx, export)."""
     vectors = (pre_weight, pre_bias, post_weight, post_bias, scale)
     if _lib.TRACE is None and not any(hasattr(v, '_ss_grad_ready') for v in vectors):
         if post not in ops._NORM or pre not in ops._NORM or gate_act not in ops._GATE_ACT:

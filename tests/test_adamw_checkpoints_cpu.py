@@ -101,3 +101,26 @@ def test_a_refused_checkpoint_changes_nothing(bits):
         refused(opt, spoil(f), match)
     opt.load_state_dict(good)
     assert (opt.lr, opt.betas, opt.seed, opt.t) == (1e-3, (0.9, 0.999), 9, 0) and not opt.exp_avg[:16].any()
+
+
+def test_a_checkpoint_with_parameters_that_are_frozen_here():
+    """torch was given all parameters, the first of them frozen: its numbers are not those of the trainable ones"""
+    net = nets()
+    net[0].weight.requires_grad_(False)
+    net[0].weight.grad = None
+    ref = torch.optim.AdamW(net.parameters(), lr=2e-3, weight_decay=0.1)
+    ref.step()
+    trainable = [p for p in net.parameters() if p.requires_grad]
+    opt = AdamW(trainable)
+    refused(opt, ref.state_dict(), 'order')
+    opt.load_state_dict(ref.state_dict(), order=net.parameters())
+    for i, p in enumerate(trainable):
+        assert torch.equal(opt.state_dict()['state'][i]['exp_avg'], ref.state[p]['exp_avg'])
+
+
+def test_codes_of_another_type_are_refused():
+    net = nets()
+    opt = AdamW(net.parameters(), state_bits=8)
+    sd = opt.state_dict()
+    sd['state'][2]['exp_avg_sq'] = sd['state'][2]['exp_avg_sq'].to(torch.int8)
+    refused(opt, sd, 'exp_avg_sq')
